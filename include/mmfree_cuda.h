@@ -73,11 +73,14 @@ int mmfree_cuda_bitlinear(float* out, const float* x, const float* norm_weight,
                           int frac_bits, int32_t* acc_out, void* stream);
 
 /* Status of the asynchronous kernel entry points (mmfree_cuda_bitlinear,
- * mmfree_cuda_bitlinear_cluster, mmfree_cuda_bitlinear_noalloc). They return once their
- * kernels are queued; a failure inside a kernel (a bounded wait that gave up) is recorded in
+ * mmfree_cuda_bitlinear_cluster, mmfree_cuda_bitlinear_noalloc, mmfree_cuda_causal_conv,
+ * mmfree_cuda_selective_scan and their steps). They return once their
+ * kernels are queued; a failure inside a kernel (a bounded wait that gave up, a sequence
+ * start or slot out of range) is recorded in
  * a device error word instead. This call synchronizes `stream` (the stream those calls used),
  * reads and clears the calling device's words and returns MMFREE_OK, or MMFREE_E_TIMEOUT when
- * a call since the last check failed -- the outputs of those calls are then undefined. It
+ * a call since the last check failed -- the outputs of those calls are then undefined -- or
+ * MMFREE_E_RANGE when one met a bad sequence start or slot. It
  * allocates nothing. No reference counterpart: the reference kernels are synchronous host
  * code that cannot time out. */
 int mmfree_cuda_kernel_status(void* stream);
@@ -167,6 +170,105 @@ int mmfree_cuda_hgrn_scan(float* out, const float* i, const float* f, size_t T, 
 int mmfree_cuda_rmsnorm_swishgate(float* out, const float* g, const float* o,
                                   const float* weight, size_t rows, size_t cols, float eps,
                                   void* stream);
+
+/* ---- recurrent-block operators (device pointers) --------------------------------------
+ * The operators of a block whose token mixer is a selective state space scan, beside the
+ * HGRN ones above, for prompts (sequences packed one behind another without padding) and for
+ * single tokens. No reference counterpart: the reference's only mixer is the HGRN scan, and
+ * its `use_short_conv` flag (config.hpp:15) has no kernel behind it.
+ *
+ * Types are MMFREE_T_*. `ld*` are row pitches in elements; the elements of a row are
+ * contiguous. Outputs must not overlap inputs. The calls use no workspace, allocate nothing
+ * and may be captured; calls on different streams do not disturb each other as long as they
+ * write different buffers and states.
+ *
+ * Sequences: seq_starts (device, seqs + 1 ascending values in [0, tokens]) gives the first
+ * row of each sequence and the row behind the last one; rows outside are not read and their
+ * outputs are left as they were; an empty sequence leaves its state as it was. NULL means one
+ * sequence of all tokens (seqs must be 1). slots (device, nullable: sequence s uses state
+ * s): the state each sequence reads and updates, out of slot_count; the slots of one call
+ * must differ. A negative slot marks a sequence that is not there (a padded batch): its
+ * outputs and every state are left as they were. Values of seq_starts or slots that break
+ * these rules make the kernel skip the sequence and record it: mmfree_cuda_kernel_status
+ * then returns MMFREE_E_RANGE. */
+enum { MMFREE_T_F32 = 0, MMFREE_T_BF16 = 1, MMFREE_T_F16 = 2, MMFREE_T_S8 = 3, MMFREE_T_E4M3 = 4 };
+
+#define MMFREE_CUDA_MAX_STATES 256  /* state dimension of the selective scan */
+#define MMFREE_CUDA_MAX_CONV_WIDTH 8
+
+/* r = residual + x, rounded to `type` and stored back into residual (NULL: r = x); then the
+ * RMS norm of r with `weight`, as 8-bit codes with scales: norm(r) ~ codes * scale.
+ *   t = r * weight (rounded to fp32), m = max |t| over the row, or over each `group` columns
+ *   MMFREE_T_S8:   code = t * 127 / m, the exact quotient rounded half to even
+ *   MMFREE_T_E4M3: code = e4m3(t * (448 / m))
+ *   scale = m / (127 or 448) / sqrt(mean(r^2) + eps)
+ * x [rows, cols] and residual of `type` (F32, BF16 or F16); codes [rows, cols] and scales
+ * [rows, ceil(cols / group)] contiguous; group 0 (one scale a row), 32, 64 or 128. A row of
+ * zeros has codes and scale 0; a row with a NaN or an infinity has NaN scales. */
+int mmfree_cuda_add_rmsnorm_quant(void* codes, float* scales, const void* x, size_t ldx,
+                                  void* residual, size_t ld_res, const float* weight,
+                                  size_t rows, size_t cols, float eps, int type, int code_type,
+                                  size_t group, void* stream);
+
+/* out[m, n] = x_scales[m] * sum_k x[m, k] * (u[n, k] - zero[n, k / group]) * scale[n, k / group]
+ * for 4-bit weights u in 0..15. codes: [out_dim, ceil(in_dim / 2)] bytes with row pitch
+ * ld_codes bytes, element 2j in the low and 2j + 1 in the high half of byte j; scales
+ * [out_dim, ceil(in_dim / group)] of scale_type (F32, BF16 or F16) and zeros (uint8, same
+ * shape; NULL: 8) contiguous; group a multiple of 32. x [rows, in_dim] of x_type: F32, BF16
+ * or F16 with x_scales NULL, or S8 / E4M3 codes with the scales of
+ * mmfree_cuda_add_rmsnorm_quant: x_scales [rows] with x_group 0, or [rows, ceil(in_dim /
+ * group)] with x_group == group. out [rows, out_dim] contiguous of out_type (F32, BF16 or
+ * F16). Sums are in fp32. Meant for a few rows (1 to 32), right for any number. */
+int mmfree_cuda_int4_matvec(void* out, const void* x, size_t ldx, const float* x_scales,
+                            const uint8_t* codes, size_t ld_codes, const void* scales,
+                            const uint8_t* zeros, size_t rows, size_t in_dim, size_t out_dim,
+                            size_t group, size_t x_group, int x_type, int scale_type,
+                            int out_type, void* stream);
+
+typedef struct {
+  void* out;             /* [tokens, channels] of `type` */
+  const void* x;         /* [tokens, channels] */
+  const float* weight;   /* [channels, width], the newest input's tap last */
+  const float* bias;     /* [channels] (nullable) */
+  void* state;           /* [slot_count, width - 1, channels] of `type`, the inputs before the
+                            sequence, oldest first; updated (nullable: zeros, not kept) */
+  const int32_t* seq_starts;
+  const int32_t* slots;
+  size_t ld_out, ldx, tokens, seqs, slot_count, channels, width; /* width 2..8 */
+  int type, silu;
+} mmfree_cuda_conv_args;
+
+/* The short causal convolution of each channel: out[t, d] = bias[d] + sum_j weight[d, j] *
+ * in[t - (width - 1) + j, d], through x * sigmoid(x) when silu is set. */
+int mmfree_cuda_causal_conv(const mmfree_cuda_conv_args* a, void* stream);
+/* The same for one token of each of `seqs` streams (tokens = seqs, seq_starts ignored). */
+int mmfree_cuda_causal_conv_step(const mmfree_cuda_conv_args* a, void* stream);
+
+typedef struct {
+  void* out;             /* [tokens, channels] of `type` */
+  const void* x;         /* [tokens, channels] */
+  const void* dt;        /* [tokens, channels] */
+  const void* z;         /* [tokens, channels] (nullable: no gate) */
+  const void* B;         /* [tokens, groups, states]: channel d uses group d / (channels / groups) */
+  const void* C;         /* [tokens, groups, states] */
+  const float* A;        /* [channels, states] */
+  const float* D;        /* [channels] (nullable) */
+  const float* dt_bias;  /* [channels] (nullable) */
+  float* state;          /* [slot_count, channels, states]; updated (nullable in a scan: zeros,
+                            not kept) */
+  const int32_t* seq_starts;
+  const int32_t* slots;
+  size_t ld_out, ldx, ld_dt, ldz, ldb, ldc;
+  size_t tokens, seqs, slot_count, channels, states, groups;
+  int type;
+  int dt_softplus;       /* delta = softplus(dt + dt_bias), else dt + dt_bias */
+} mmfree_cuda_ssm_args;
+
+/* The selective scan: h = exp(delta * A) * h + delta * x * B (state, fp32), out = (C . h +
+ * D * x) * z * sigmoid(z), token after token of each sequence. */
+int mmfree_cuda_selective_scan(const mmfree_cuda_ssm_args* a, void* stream);
+/* The same for one token of each of `seqs` streams (tokens = seqs, seq_starts ignored). */
+int mmfree_cuda_selective_step(const mmfree_cuda_ssm_args* a, void* stream);
 
 /* ---- model (host buffers) ------------------------------------------------------------ */
 typedef struct mmfree_cuda_model mmfree_cuda_model;

@@ -5,6 +5,7 @@ The product is ``_lib/libmmfree_cuda.so`` (CUDA kernels + the C ABI of
 the reference's C++ API in Python (``api``) and writes seeded ``model.mmfree`` blobs
 (``blob``).
 """
-from .api import (Config, Model, MmfreeError, bitlinear, bitlinear_cluster, hgrn_scan,  # noqa: F401
-                  pack_ternary_host, packed_bytes, repack_ternary, rmsnorm,
-                  rmsnorm_swishgate, swiglu, ternary_matmul)
+from .api import (Config, Model, MmfreeError, add_rmsnorm_quant, bitlinear,  # noqa: F401
+                  bitlinear_cluster, causal_conv, causal_conv_step, hgrn_scan, int4_matvec,
+                  pack_ternary_host, packed_bytes, repack_ternary, rmsnorm, rmsnorm_swishgate,
+                  selective_scan, selective_step, swiglu, ternary_matmul)

@@ -15,6 +15,7 @@ LIB_PATH = _build.LIB
 OK = 0
 E_INVALID, E_CUDA, E_IO, E_RANGE, E_STATE, E_INTERNAL, E_TIMEOUT = -1, -2, -3, -4, -5, -6, -7
 ACT_FLOAT, ACT_FIXED_Q510 = 0, 1
+T_F32, T_BF16, T_F16, T_S8, T_E4M3 = range(5)
 MAX_IN_DIM = 57344
 
 VP, SZ, F, I, I64, U64 = C.c_void_p, C.c_size_t, C.c_float, C.c_int, C.c_int64, C.c_uint64
@@ -39,6 +40,12 @@ SIGNATURES = {
     "mmfree_cuda_swiglu": (I, [VP, VP, VP, SZ, VP]),
     "mmfree_cuda_hgrn_scan": (I, [VP, VP, VP, SZ, SZ, VP, VP]),
     "mmfree_cuda_rmsnorm_swishgate": (I, [VP, VP, VP, VP, SZ, SZ, F, VP]),
+    "mmfree_cuda_add_rmsnorm_quant": (I, [VP, VP, VP, SZ, VP, SZ, VP, SZ, SZ, F, I, I, SZ, VP]),
+    "mmfree_cuda_int4_matvec": (I, [VP, VP, SZ, VP, VP, SZ, VP, VP, SZ, SZ, SZ, SZ, SZ, I, I, I, VP]),
+    "mmfree_cuda_causal_conv": (I, [VP, VP]),
+    "mmfree_cuda_causal_conv_step": (I, [VP, VP]),
+    "mmfree_cuda_selective_scan": (I, [VP, VP]),
+    "mmfree_cuda_selective_step": (I, [VP, VP]),
     "mmfree_cuda_model_open": (I, [C.c_char_p, I, I, I, C.POINTER(VP)]),
     "mmfree_cuda_model_close": (None, [VP]),
     "mmfree_cuda_nccl_unique_id": (I, [VP]),
@@ -65,6 +72,20 @@ SIGNATURES = {
 class KernelStats(C.Structure):
     _fields_ = [("name", C.c_char_p), ("ms", C.c_double), ("launches", C.c_int64),
                 ("bytes", C.c_double), ("ops", C.c_double)]
+
+
+class ConvArgs(C.Structure):
+    _fields_ = [(n, VP) for n in ("out", "x", "weight", "bias", "state", "seq_starts", "slots")] + \
+               [(n, SZ) for n in ("ld_out", "ldx", "tokens", "seqs", "slot_count", "channels", "width")] + \
+               [("type", I), ("silu", I)]
+
+
+class SsmArgs(C.Structure):
+    _fields_ = [(n, VP) for n in ("out", "x", "dt", "z", "B", "C", "A", "D", "dt_bias", "state",
+                                  "seq_starts", "slots")] + \
+               [(n, SZ) for n in ("ld_out", "ldx", "ld_dt", "ldz", "ldb", "ldc", "tokens", "seqs",
+                                  "slot_count", "channels", "states", "groups")] + \
+               [("type", I), ("dt_softplus", I)]
 
 
 class MmfreeError(RuntimeError):

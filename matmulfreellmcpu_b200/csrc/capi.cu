@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "../../include/mmfree_cuda.h"
+#include "block_ops.h"
 #include "common.cuh"
 #include "kernels.h"
 #include "blob.h"
@@ -416,9 +417,15 @@ int mmfree_cuda_kernel_status(void* stream) {
     }
     if (arena) f |= take_flags(reinterpret_cast<uint32_t*>(arena) + kAsyncFlagWord, st);
     if (char* head = noalloc_base_if_ready(dev)) f |= take_flags(reinterpret_cast<uint32_t*>(head), st);
+    uint32_t sequence = 0;
+    ck(take_sequence_flags(st, &sequence), "reading the sequence error word");
+    f |= sequence;
     if (f & kErrTimeout)
       throw TimeoutError("a bounded wait inside a BitLinear kernel gave up: the outputs of the "
                          "kernel calls since the last status check are undefined");
+    if (f & kErrRange)
+      throw std::out_of_range("a sequence start or slot given to causal_conv or selective_scan "
+                              "since the last status check is out of range or out of order");
     if (f) throw std::runtime_error("device error flag set");
   });
 }
@@ -465,6 +472,150 @@ int mmfree_cuda_ternary_matmul(int32_t* acc, const int32_t* x, const void* wpack
     ck(launch_matmul(a, st), "matmul kernel");
     check_flags(flags, st);
   });
+}
+
+// ---- recurrent-block operators --------------------------------------------------------------
+}  // extern "C"
+
+namespace {
+
+bool row_type(int t) { return t == MMFREE_T_F32 || t == MMFREE_T_BF16 || t == MMFREE_T_F16; }
+
+constexpr size_t kMaxDim = size_t(1) << 30;
+
+// need() whose message names the entry point (put together only on failure).
+void need_in(const char* what, bool ok, const char* message) {
+  if (!ok) throw std::invalid_argument(std::string(what) + ": " + message);
+}
+
+// The common checks of a call over packed sequences; false: there is nothing to compute.
+bool check_sequences(const char* what, bool step, size_t tokens, size_t seqs, size_t channels,
+                     const void* state, const int32_t* seq_starts, const int32_t* slots,
+                     size_t slot_count) {
+  need_in(what, channels > 0 && channels <= kMaxDim, "channels must be in [1, 2^30]");
+  need_in(what, tokens <= kMaxDim, "more than 2^30 tokens");
+  need_in(what, seqs <= 65535, "more than 65535 sequences");
+  need_in(what, !step || tokens == seqs, "a step has one token a stream");
+  need_in(what, step || seq_starts || seqs == 1, "seqs must be 1 without seq_starts");
+  need_in(what, !slots || state, "slots without a state");
+  need_in(what, slots || slot_count >= seqs || !state, "fewer states than sequences");
+  need_in(what, slot_count <= kMaxDim, "more than 2^30 slots");
+  return tokens > 0 && seqs > 0;
+}
+
+void check_conv(const char* what, const mmfree_cuda_conv_args* a, bool step, void* stream) {
+  need(a != nullptr, "null arguments");
+  need_in(what, row_type(a->type), "type must be F32, BF16 or F16");
+  need_in(what, a->width >= 2 && a->width <= MMFREE_CUDA_MAX_CONV_WIDTH, "width must be 2..8");
+  mmfree_cuda_conv_args c = *a;
+  if (step) c.seq_starts = nullptr;
+  if (!check_sequences(what, step, c.tokens, c.seqs, c.channels, c.state, c.seq_starts, c.slots, c.slot_count)) return;
+  need_in(what, c.out && c.x && c.weight, "null pointer");
+  need_in(what, c.ld_out >= c.channels || c.tokens == 1, "output rows overlap");
+  if (!c.state) c.slot_count = c.seqs;
+  ck(step ? launch_causal_conv_step(c, as_stream(stream)) : launch_causal_conv(c, as_stream(stream)), what);
+}
+
+void check_ssm(const char* what, const mmfree_cuda_ssm_args* a, bool step, void* stream) {
+  need(a != nullptr, "null arguments");
+  need_in(what, row_type(a->type), "type must be F32, BF16 or F16");
+  need_in(what, a->states >= 1 && a->states <= MMFREE_CUDA_MAX_STATES, "states must be 1..256");
+  need_in(what, a->groups >= 1 && a->channels % a->groups == 0, "groups must divide channels");
+  mmfree_cuda_ssm_args c = *a;
+  if (step) c.seq_starts = nullptr;
+  if (!check_sequences(what, step, c.tokens, c.seqs, c.channels, c.state, c.seq_starts, c.slots, c.slot_count)) return;
+  need_in(what, c.out && c.x && c.dt && c.B && c.C && c.A, "null pointer");
+  need_in(what, !step || c.state, "a step needs a state");
+  need_in(what, c.ld_out >= c.channels || c.tokens == 1, "output rows overlap");
+  if (!c.state) c.slot_count = c.seqs;
+  ck(step ? launch_selective_step(c, as_stream(stream)) : launch_selective_scan(c, sm_count_of_device(), as_stream(stream)),
+     what);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mmfree_cuda_add_rmsnorm_quant(void* codes, float* scales, const void* x, size_t ldx,
+                                  void* residual, size_t ld_res, const float* weight,
+                                  size_t rows, size_t cols, float eps, int type, int code_type,
+                                  size_t group, void* stream) {
+  return guard([&] {
+    need(row_type(type), "add_rmsnorm_quant: type must be F32, BF16 or F16");
+    need(code_type == MMFREE_T_S8 || code_type == MMFREE_T_E4M3, "add_rmsnorm_quant: code_type must be S8 or E4M3");
+    need(group == 0 || group == 32 || group == 64 || group == 128, "add_rmsnorm_quant: group must be 0, 32, 64 or 128");
+    need(cols >= 1 && cols <= MMFREE_CUDA_MAX_IN_DIM, "add_rmsnorm_quant: cols must be in [1, MMFREE_CUDA_MAX_IN_DIM]");
+    need(rows <= kMaxDim, "add_rmsnorm_quant: more than 2^30 rows");
+    if (rows == 0) return;
+    need(codes && scales && x && weight, "add_rmsnorm_quant: null pointer");
+    need(!residual || ld_res >= cols || rows == 1, "add_rmsnorm_quant: residual rows overlap");
+    NormQuantArgs a;
+    a.codes = codes;
+    a.scales = scales;
+    a.x = x;
+    a.residual = residual;
+    a.weight = weight;
+    a.rows = static_cast<int64_t>(rows);
+    a.ldx = static_cast<int64_t>(ldx);
+    a.ldr = static_cast<int64_t>(ld_res);
+    a.cols = static_cast<int>(cols);
+    a.group = static_cast<int>(group);
+    a.parts = group ? static_cast<int>((cols + group - 1) / group) : 1;
+    a.eps = eps;
+    a.type = type;
+    a.code_type = code_type;
+    ck(launch_norm_quant(a, as_stream(stream)), "norm_quant kernel");
+  });
+}
+
+int mmfree_cuda_int4_matvec(void* out, const void* x, size_t ldx, const float* x_scales,
+                            const uint8_t* codes, size_t ld_codes, const void* scales,
+                            const uint8_t* zeros, size_t rows, size_t in_dim, size_t out_dim,
+                            size_t group, size_t x_group, int x_type, int scale_type,
+                            int out_type, void* stream) {
+  return guard([&] {
+    check_dims(rows, in_dim, out_dim);
+    need(row_type(x_type) || x_type == MMFREE_T_S8 || x_type == MMFREE_T_E4M3, "int4_matvec: bad x_type");
+    need(row_type(scale_type) && row_type(out_type), "int4_matvec: scale_type and out_type must be F32, BF16 or F16");
+    need(group >= 32 && group % 32 == 0 && group <= kMaxDim, "int4_matvec: group must be a multiple of 32");
+    need(row_type(x_type) == (x_scales == nullptr), "int4_matvec: x_scales go with 8-bit rows, and only with them");
+    need(x_group == 0 || (x_group == group && x_scales), "int4_matvec: x_group must be 0 or the weights' group");
+    if (rows == 0) return;
+    need(out && x && codes && scales, "int4_matvec: null pointer");
+    need(ld_codes >= (in_dim + 1) / 2 || out_dim == 1, "int4_matvec: ld_codes is less than a row");
+    Int4Args a;
+    a.out = out;
+    a.x = x;
+    a.x_scales = x_scales;
+    a.codes = codes;
+    a.scales = scales;
+    a.zeros = zeros;
+    a.ldx = static_cast<int64_t>(ldx);
+    a.ldw = static_cast<int64_t>(ld_codes);
+    a.M = static_cast<int>(rows);
+    a.N = static_cast<int>(out_dim);
+    a.K = static_cast<int>(in_dim);
+    a.group = static_cast<int>(group);
+    a.parts = static_cast<int>((in_dim + group - 1) / group);
+    a.x_grouped = x_group != 0;
+    a.x_type = x_type;
+    a.scale_type = scale_type;
+    a.out_type = out_type;
+    ck(launch_int4_matvec(a, sm_count_of_device(), as_stream(stream)), "int4_matvec kernel");
+  });
+}
+
+int mmfree_cuda_causal_conv(const mmfree_cuda_conv_args* a, void* stream) {
+  return guard([&] { check_conv("causal_conv", a, false, stream); });
+}
+int mmfree_cuda_causal_conv_step(const mmfree_cuda_conv_args* a, void* stream) {
+  return guard([&] { check_conv("causal_conv_step", a, true, stream); });
+}
+int mmfree_cuda_selective_scan(const mmfree_cuda_ssm_args* a, void* stream) {
+  return guard([&] { check_ssm("selective_scan", a, false, stream); });
+}
+int mmfree_cuda_selective_step(const mmfree_cuda_ssm_args* a, void* stream) {
+  return guard([&] { check_ssm("selective_step", a, true, stream); });
 }
 
 // ---- TernaryBackend seam over host buffers ------------------------------------------------

@@ -1,0 +1,61 @@
+// elements.cuh -- fp32, bf16 and fp16 rows read and written as fp32 registers.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+namespace mmfree_cuda {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// V consecutive elements as they lie in memory, at most 16 bytes per access.
+template <typename T, int V>
+struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
+  T v[V];
+};
+
+// V elements from a 16-byte aligned address (kVec), or the first n of them one by one.
+template <bool kVec, typename T, int V>
+__device__ __forceinline__ void load_row(const T* p, int n, float (&r)[V]) {
+  if constexpr (kVec) {
+    const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = to_f32(k.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = i < n ? to_f32(p[i]) : 0.0f;
+  }
+}
+
+template <bool kVec, typename T, int V>
+__device__ __forceinline__ void store_row(T* p, int n, const float (&r)[V]) {
+  if constexpr (kVec) {
+    Pack<T, V> k;
+#pragma unroll
+    for (int i = 0; i < V; ++i) k.v[i] = from_f32<T>(r[i]);
+    *reinterpret_cast<Pack<T, V>*>(p) = k;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) p[i] = from_f32<T>(r[i]);
+  }
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+__device__ __forceinline__ float silu_f32(float v) { return v / (1.0f + expf(-v)); }
+
+}  // namespace mmfree_cuda
