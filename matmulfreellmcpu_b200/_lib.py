@@ -114,6 +114,27 @@ def lib() -> C.CDLL:
     return _LIB
 
 
+_BIND = None
+
+
+def bind():
+    """Load the extension that calls the library on torch tensors (once); raises if missing."""
+    global _BIND
+    if _BIND is None:
+        lib()  # the library it links
+        import torch  # noqa: F401  (its shared libraries must be loaded first)
+        from importlib.machinery import ExtensionFileLoader
+        from importlib.util import module_from_spec, spec_from_file_location
+        if not os.path.exists(_build.BIND):
+            raise ImportError(f"{_build.BIND} is missing: run `python -m matmulfreellmcpu_b200.build`")
+        loader = ExtensionFileLoader("mmfree_tensor_ops", _build.BIND)
+        m = module_from_spec(spec_from_file_location("mmfree_tensor_ops", _build.BIND, loader=loader))
+        loader.exec_module(m)
+        m.set_error(MmfreeError)
+        _BIND = m
+    return _BIND
+
+
 def check(rc: int) -> None:
     if rc != OK:
         raise MmfreeError(rc, lib().mmfree_cuda_last_error().decode(errors="replace"))

@@ -16,8 +16,8 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from ._lib import (ACT_FIXED_Q510, ACT_FLOAT, E_INVALID, T_BF16, T_E4M3, T_F16, T_F32,  # noqa: F401
-                   T_S8, ConvArgs, MmfreeError, SsmArgs, check, lib)
+from ._lib import (ACT_FIXED_Q510, ACT_FLOAT, E_INVALID, MmfreeError, bind, check,  # noqa: F401
+                   lib)
 
 ActQuant = {"float": ACT_FLOAT, "fixed": ACT_FIXED_Q510}
 
@@ -348,95 +348,9 @@ def rmsnorm_swishgate(g, o, weight, eps: float = 1e-6, stream=None):
 # ---- operators of a recurrent block ------------------------------------------------------------
 # Rows may be slices of wider rows (any row pitch, contiguous elements). With ``stream`` the
 # call runs on that stream and its outputs belong to it, as torch tensors made under
-# ``torch.cuda.stream(stream)`` do; without, on the tensors' device's current stream.
-
-_TYPES: dict = {}
-
-
-def _type_of(dtype) -> int | None:
-    if not _TYPES:
-        import torch
-        _TYPES.update({torch.float32: T_F32, torch.bfloat16: T_BF16, torch.float16: T_F16,
-                       torch.int8: T_S8, torch.float8_e4m3fn: T_E4M3})
-    return _TYPES.get(dtype)
-
-
-def _need(ok, what: str) -> None:
-    if not ok:
-        raise MmfreeError(E_INVALID, what)
-
-
-def _row_type(t, name: str) -> int:
-    code = _type_of(t.dtype)
-    _need(code is not None and code <= T_F16, f"{name} must be float32, bfloat16 or float16")
-    return code
-
-
-def _pitch(t, name: str, rows: int, cols: int, dtype, device) -> int:
-    """Row pitch of a [rows, cols] operand, checked."""
-    _need(t.device == device, f"{name} is on {t.device}, not on {device}")
-    _need(t.dtype == dtype, f"{name} must be {dtype}, not {t.dtype}")
-    _need(t.dim() == 2 and t.shape[0] == rows and t.shape[1] == cols,
-          f"{name} must be [{rows}, {cols}], not {list(t.shape)}")
-    s = t.stride()
-    _need(s[1] == 1 or cols <= 1, f"{name}'s rows must be contiguous")
-    return s[0]
-
-
-def _dense(t, name: str, shape: tuple, dtype, device) -> None:
-    _need(t.device == device, f"{name} is on {t.device}, not on {device}")
-    _need(t.dtype == dtype, f"{name} must be {dtype}, not {t.dtype}")
-    _need(tuple(t.shape) == shape and t.is_contiguous(),
-          f"{name} must be a contiguous {list(shape)}, not {list(t.shape)}")
-
-
-def _span(t) -> tuple[int, int]:
-    """The bytes from a tensor's first to behind its last element."""
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size() if t.numel() else t.data_ptr()
-
-
-def _apart(a, a_name: str, b, b_name: str) -> None:
-    if b is not None:
-        (a0, a1), (b0, b1) = _span(a), _span(b)
-        _need(a1 <= b0 or b1 <= a0, f"{a_name} overlaps {b_name}")
-
-
-class _On:
-    """The device and stream of one call: makes its outputs there and runs the entry point."""
-
-    __slots__ = ("device", "stream", "other")
-
-    def __init__(self, x, stream):
-        import torch
-        _need(x.is_cuda, "the tensors must be on a CUDA device")
-        self.device = x.device
-        self.other = stream
-        if stream is None:
-            self.stream = torch.cuda.current_stream(self.device).cuda_stream
-        else:
-            _need(stream.device == self.device, f"the stream is on {stream.device}, not on {self.device}")
-            self.stream = stream.cuda_stream
-
-    def empty(self, *shape, dtype):
-        import torch
-        if self.other is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
-        with torch.cuda.stream(self.other):
-            return torch.empty(shape, dtype=dtype, device=self.device)
-
-    def run(self, entry, *args, held=()) -> None:
-        import torch
-        if self.other is not None:  # the caller's allocator streams may differ from this one
-            for t in held:
-                if t is not None:
-                    t.record_stream(self.other)
-        if torch.cuda.current_device() == self.device.index:
-            check(entry(*args, self.stream))
-        else:
-            with torch.cuda.device(self.device):
-                check(entry(*args, self.stream))
-
+# ``torch.cuda.stream(stream)`` do; without, on the current stream of the tensors' device.
+# bind/tensor_ops.cpp checks the tensors and makes the outputs. There is no backward pass: an
+# input that requires a gradient is refused while gradients are recorded.
 
 def add_rmsnorm_quant(x, weight, residual=None, eps: float = 1e-6, code: str = "int8", group: int = 0,
                       stream=None):
@@ -447,26 +361,9 @@ def add_rmsnorm_quant(x, weight, residual=None, eps: float = 1e-6, code: str = "
     ``code``: "int8" (the exact quotient by the scale, half to even) or "e4m3"
     (torch.float8_e4m3fn). ``group``: columns of a scale, 32, 64 or 128, or 0 for one scale a
     row; ``scales`` is float32 [rows, ceil(cols / group)], a row's [rows, 1]."""
-    import torch
-    kind = _row_type(x, "x")
-    _need(x.dim() == 2, "x must be [rows, cols]")
-    rows, cols = x.shape
-    on = _On(x, stream)
-    ldx = _pitch(x, "x", rows, cols, x.dtype, on.device)
-    _dense(weight, "weight", (cols,), torch.float32, on.device)
-    _need(code in ("int8", "e4m3"), "code must be 'int8' or 'e4m3'")
-    _need(group in (0, 32, 64, 128), "group must be 0, 32, 64 or 128")
-    ldr = 0
-    if residual is not None:
-        ldr = _pitch(residual, "residual", rows, cols, x.dtype, on.device)
-        _apart(residual, "residual", x, "x")
-        _apart(residual, "residual", weight, "weight")
-    codes = on.empty(rows, cols, dtype=torch.int8 if code == "int8" else torch.float8_e4m3fn)
-    scales = on.empty(rows, -(-cols // group) if group else 1, dtype=torch.float32)
-    on.run(lib().mmfree_cuda_add_rmsnorm_quant, codes.data_ptr(), scales.data_ptr(), x.data_ptr(), ldx,
-           _ptr(residual), ldr, weight.data_ptr(), rows, cols, eps, kind,
-           T_S8 if code == "int8" else T_E4M3, group, held=(x, residual, weight))
-    return codes, scales
+    if code not in ("int8", "e4m3"):
+        raise MmfreeError(E_INVALID, "code must be 'int8' or 'e4m3'")
+    return bind().add_rmsnorm_quant(x, weight, residual, eps, code == "int8", group, stream)
 
 
 def int4_matvec(x, codes, scales, group: int, zeros=None, x_scales=None, out_dtype=None, stream=None):
@@ -479,83 +376,7 @@ def int4_matvec(x, codes, scales, group: int, zeros=None, x_scales=None, out_dty
     codes of :func:`add_rmsnorm_quant` with its scales as ``x_scales`` (one a row, or of the
     same ``group``). Returns [rows, out_dim] of ``out_dtype`` (``x``'s type; float32 for codes).
     Row pitches of ``codes`` that are multiples of 16 bytes are the fast ones."""
-    import torch
-    kind = _type_of(x.dtype)
-    _need(kind is not None, "x must be float32, bfloat16, float16, int8 or float8_e4m3fn")
-    _need(x.dim() == 2 and codes.dim() == 2, "x and codes must have two dimensions")
-    rows, in_dim = x.shape
-    out_dim = codes.shape[0]
-    on = _On(x, stream)
-    ldx = _pitch(x, "x", rows, in_dim, x.dtype, on.device)
-    ldw = _pitch(codes, "codes", out_dim, (in_dim + 1) // 2, torch.uint8, on.device)
-    _need(group >= 32 and group % 32 == 0, "group must be a multiple of 32")
-    parts = -(-in_dim // group)
-    scale_kind = _row_type(scales, "scales")
-    _dense(scales, "scales", (out_dim, parts), scales.dtype, on.device)
-    if zeros is not None:
-        _dense(zeros, "zeros", (out_dim, parts), torch.uint8, on.device)
-    _need((x_scales is not None) == (kind >= T_S8), "x_scales go with 8-bit rows, and only with them")
-    x_group = 0
-    if x_scales is not None:
-        if x_scales.dim() == 2 and x_scales.shape[1] == parts and parts > 1:
-            x_group = group
-        _dense(x_scales, "x_scales", (rows, parts if x_group else 1), torch.float32, on.device)
-    if out_dtype is None:
-        out_dtype = x.dtype if kind <= T_F16 else torch.float32
-    out = on.empty(rows, out_dim, dtype=out_dtype)
-    on.run(lib().mmfree_cuda_int4_matvec, out.data_ptr(), x.data_ptr(), ldx, _ptr(x_scales),
-           codes.data_ptr(), ldw, scales.data_ptr(), _ptr(zeros), rows, in_dim, out_dim, group, x_group,
-           kind, scale_kind, _row_type(out, "out_dtype"), held=(x, codes, scales, zeros, x_scales))
-    return out
-
-
-def _sequences(on, rows: int, seq_starts, slots, state, step: bool) -> tuple[int, int]:
-    """(sequences, states) of a call over packed rows, checked."""
-    import torch
-    if step:
-        seqs = rows
-    elif seq_starts is None:
-        seqs = 1
-    else:
-        _need(seq_starts.dim() == 1 and seq_starts.shape[0] >= 1, "seq_starts must be [sequences + 1]")
-        seqs = seq_starts.shape[0] - 1
-        _dense(seq_starts, "seq_starts", (seqs + 1,), torch.int32, on.device)
-    if slots is not None:
-        _need(state is not None, "slots need a state")
-        _dense(slots, "slots", (seqs,), torch.int32, on.device)
-    count = seqs if state is None else state.shape[0]
-    _need(slots is not None or count >= seqs, f"{count} states for {seqs} sequences")
-    return seqs, count
-
-
-def _causal_conv(x, weight, bias, state, seq_starts, slots, silu, out, stream, step):
-    import torch
-    kind = _row_type(x, "x")
-    _need(x.dim() == 2 and weight.dim() == 2, "x and weight must have two dimensions")
-    rows, channels = x.shape
-    width = weight.shape[1]
-    on = _On(x, stream)
-    ldx = _pitch(x, "x", rows, channels, x.dtype, on.device)
-    _need(2 <= width <= 8, "weight must be [channels, 2 to 8]")
-    _dense(weight, "weight", (channels, width), torch.float32, on.device)
-    if bias is not None:
-        _dense(bias, "bias", (channels,), torch.float32, on.device)
-    if state is not None:
-        _need(state.dim() == 3, "state must be [states, width - 1, channels]")
-        _dense(state, "state", (state.shape[0], width - 1, channels), x.dtype, on.device)
-        _apart(state, "state", x, "x")
-    seqs, count = _sequences(on, rows, seq_starts, slots, state, step)
-    if out is None:
-        out = on.empty(rows, channels, dtype=x.dtype)
-    else:
-        for t, name in ((x, "x"), (weight, "weight"), (bias, "bias"), (state, "state")):
-            _apart(out, "out", t, name)
-    a = ConvArgs(out.data_ptr(), x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(state),
-                 _ptr(seq_starts), _ptr(slots), _pitch(out, "out", rows, channels, x.dtype, on.device),
-                 ldx, rows, seqs, count, channels, width, kind, int(silu))
-    on.run(lib().mmfree_cuda_causal_conv_step if step else lib().mmfree_cuda_causal_conv, C.byref(a),
-           held=(out, x, weight, bias, state, seq_starts, slots))
-    return out
+    return bind().int4_matvec(x, codes, scales, group, zeros, x_scales, out_dtype, stream)
 
 
 def causal_conv(x, weight, bias=None, state=None, seq_starts=None, slots=None, silu: bool = False,
@@ -571,68 +392,14 @@ def causal_conv(x, weight, bias=None, state=None, seq_starts=None, slots=None, s
     oldest first, updated in place (without: zeros). ``slots`` int32 [sequences]: the state of
     each sequence (they must differ; a negative one marks a sequence that is left out).
     Starts or slots out of range are reported by :func:`kernel_status`."""
-    return _causal_conv(x, weight, bias, state, seq_starts, slots, silu, out, stream, False)
+    return bind().causal_conv(x, weight, bias, state, seq_starts, slots, silu, out, stream, False)
 
 
 def causal_conv_step(x, weight, state, bias=None, slots=None, silu: bool = False, out=None,
                      stream=None):
     """:func:`causal_conv` for one token of each stream: row s of ``x`` continues the sequence
     whose inputs are in state ``slots[s]`` (s without ``slots``)."""
-    _need(state is not None, "a step needs a state")
-    return _causal_conv(x, weight, bias, state, None, slots, silu, out, stream, True)
-
-
-def _selective(x, dt, A, B, C_, D, z, dt_bias, dt_softplus, state, seq_starts, slots, out, stream,
-               step):
-    import torch
-    kind = _row_type(x, "x")
-    _need(x.dim() == 2 and A.dim() == 2, "x and A must have two dimensions")
-    rows, channels = x.shape
-    states = A.shape[1]
-    on = _On(x, stream)
-    dev = on.device
-    ldx = _pitch(x, "x", rows, channels, x.dtype, dev)
-    ld_dt = _pitch(dt, "dt", rows, channels, x.dtype, dev)
-    ldz = 0 if z is None else _pitch(z, "z", rows, channels, x.dtype, dev)
-    _need(1 <= states <= 256, "A must be [channels, 1 to 256]")
-    _dense(A, "A", (channels, states), torch.float32, dev)
-    groups = B.shape[1] if B.dim() == 3 else 1
-    _need(groups >= 1 and channels % groups == 0, f"{groups} groups do not divide {channels} channels")
-
-    def mixed(t, name):  # [rows, states] or [rows, groups, states]
-        _need(t.device == dev, f"{name} is on {t.device}, not on {dev}")
-        _need(t.dtype == x.dtype, f"{name} must be {x.dtype}, not {t.dtype}")
-        _need(tuple(t.shape) == ((rows, groups, states) if B.dim() == 3 else (rows, states)),
-              f"{name} must be [rows, states] or [rows, groups, states], not {list(t.shape)}")
-        s = t.stride()
-        _need((s[-1] == 1 or states == 1) and (groups == 1 or s[-2] == states),
-              f"{name}'s rows must be contiguous")
-        return s[0]
-
-    ldb, ldc = mixed(B, "B"), mixed(C_, "C")
-    if D is not None:
-        _dense(D, "D", (channels,), torch.float32, dev)
-    if dt_bias is not None:
-        _dense(dt_bias, "dt_bias", (channels,), torch.float32, dev)
-    if state is not None:
-        _need(state.dim() == 3, "state must be [states, channels, A's columns]")
-        _dense(state, "state", (state.shape[0], channels, states), torch.float32, dev)
-        for t, name in ((x, "x"), (dt, "dt"), (A, "A"), (B, "B"), (C_, "C"), (z, "z")):
-            _apart(state, "state", t, name)
-    seqs, count = _sequences(on, rows, seq_starts, slots, state, step)
-    if out is None:
-        out = on.empty(rows, channels, dtype=x.dtype)
-    else:
-        for t, name in ((x, "x"), (dt, "dt"), (A, "A"), (B, "B"), (C_, "C"), (z, "z"), (D, "D"),
-                        (dt_bias, "dt_bias"), (state, "state")):
-            _apart(out, "out", t, name)
-    a = SsmArgs(out.data_ptr(), x.data_ptr(), dt.data_ptr(), _ptr(z), B.data_ptr(), C_.data_ptr(),
-                A.data_ptr(), _ptr(D), _ptr(dt_bias), _ptr(state), _ptr(seq_starts), _ptr(slots),
-                _pitch(out, "out", rows, channels, x.dtype, dev), ldx, ld_dt, ldz, ldb, ldc, rows, seqs,
-                count, channels, states, groups, kind, int(dt_softplus))
-    on.run(lib().mmfree_cuda_selective_step if step else lib().mmfree_cuda_selective_scan, C.byref(a),
-           held=(out, x, dt, z, B, C_, A, D, dt_bias, state, seq_starts, slots))
-    return out
+    return bind().causal_conv(x, weight, bias, state, None, slots, silu, out, stream, True)
 
 
 def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus: bool = True,
@@ -648,13 +415,13 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus: bo
     ``D`` and ``dt_bias`` [channels] and ``state`` [states, channels, A's columns] float32, the
     state updated in place (without: zeros). ``seq_starts``, ``slots`` and ``out`` as in
     :func:`causal_conv`. Returns y of ``x``'s type."""
-    return _selective(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state, seq_starts, slots, out, stream,
-                      False)
+    return bind().selective(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state, seq_starts, slots, out,
+                            stream, False)
 
 
 def selective_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus: bool = True,
                    slots=None, out=None, stream=None):
     """:func:`selective_scan` for one token of each stream: row s continues the sequence in
     state ``slots[s]`` (s without ``slots``)."""
-    _need(state is not None, "a step needs a state")
-    return _selective(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state, None, slots, out, stream, True)
+    return bind().selective(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state, None, slots, out, stream,
+                            True)

@@ -77,6 +77,7 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     build_cli(force)
+    build_bind(force)
     return LIB
 
 
@@ -97,6 +98,34 @@ def build_cli(force: bool = False) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"cli build failed:\n{r.stdout}\n{r.stderr}")
     return CLI
+
+
+BIND = os.path.join(LIBDIR, "mmfree_tensor_ops.so")
+BIND_SRC = os.path.join(PKG, "bind", "tensor_ops.cpp")
+
+
+def build_bind(force: bool = False) -> str:
+    """The CPython extension that calls the library on torch tensors (host C++ over the C ABI and
+    the installed torch's headers, rpath to the library)."""
+    import sysconfig
+
+    import torch
+    deps = [BIND_SRC, LIB, os.path.join(INCLUDE, "mmfree_cuda.h")]
+    if force or not os.path.exists(BIND) or os.path.getmtime(BIND) < max(map(os.path.getmtime, deps)):
+        root = os.path.dirname(torch.__file__)
+        cuda = os.path.dirname(os.path.dirname(nvcc()))
+        cxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else "g++"
+        cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + INCLUDE,
+               "-isystem", os.path.join(root, "include"),
+               "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda, "include"),
+               BIND_SRC, "-L" + LIBDIR, "-lmmfree_cuda", "-L" + os.path.join(root, "lib"), "-ltorch_python",
+               "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN", "-o", BIND]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"tensor binding build failed:\n{r.stdout}\n{r.stderr}")
+    return BIND
 
 
 if __name__ == "__main__":
