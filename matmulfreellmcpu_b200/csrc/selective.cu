@@ -290,15 +290,264 @@ __global__ void __launch_bounds__(128) ssm_kernel(mmfree_cuda_ssm_args a, int la
       if (lane + j * lanes < states) state[lane + j * lanes] = h[j];
 }
 
-cudaError_t ssm_any(const mmfree_cuda_ssm_args& a, bool step, cudaStream_t s) {
+// ---- tiled scan
+
+// Two fp32 values in one 64-bit register, for the packed FMA (twice the operations an issue slot).
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+constexpr float kLog2E = 1.44269504088896341f;
+
+// softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) <= 1, with log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1/3,
+// by its series 2 (s + s^3/3 + s^5/5 + ...): the first term left out is below 2^-25 of the sum. Exact to a few
+// steps for all v, where log(1 + e) rounded first would lose small e. Two special-function operations.
+__device__ __forceinline__ float softplus_fast(float v) {
+  const float e = ex2(-fabsf(v) * kLog2E);
+  const float s = e * rcp(2.0f + e), q = s * s;
+  float p = 1.0f / 15.0f;
+  p = fmaf(p, q, 1.0f / 13.0f);
+  p = fmaf(p, q, 1.0f / 11.0f);
+  p = fmaf(p, q, 1.0f / 9.0f);
+  p = fmaf(p, q, 1.0f / 7.0f);
+  p = fmaf(p, q, 1.0f / 5.0f);
+  p = fmaf(p, q, 1.0f / 3.0f);
+  const float l = fmaf(s * q, p, s);
+  return fmaf(2.0f, l, fmaxf(v, 0.0f));
+}
+__device__ __forceinline__ float silu_fast(float v) { return v * rcp(1.0f + ex2(-v * kLog2E)); }
+
+// Sums v[i] over groups of kLanes neighbouring lanes for kSteps values at once: lane l of a group ends with the sum
+// of value l % kSteps. Each exchange halves the values a lane holds, so kSteps sums take kSteps - 1 shuffles (and
+// one for every doubling of kLanes over kSteps) instead of kSteps * log2(kLanes).
+template <int kLanes, int kSteps>
+__device__ __forceinline__ float transpose_sum(float (&v)[kSteps], int lane) {
+#pragma unroll
+  for (int o = 1; o < kSteps; o <<= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < kSteps / 2; ++i) {
+      if (i >= kSteps / (2 * o)) break;
+      // values 2i and 2i + 1 of this level go to the lanes whose bit is clear and set
+      const float keep = up ? v[2 * i + 1] : v[2 * i], send = up ? v[2 * i] : v[2 * i + 1];
+      v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, o);
+    }
+  }
+  float r = v[0];
+#pragma unroll
+  for (int o = kSteps; o < kLanes; o <<= 1) r += __shfl_xor_sync(0xFFFFFFFFu, r, o);
+  return r;
+}
+
+constexpr int kScanThreads = 128;
+
+// One CTA: kScanThreads / kLanes channels of one group and one sequence, in tiles of kTile tokens. The threads first
+// turn the tile's x and dt into (delta, delta * x) in shared memory, once per token and channel; then kLanes lanes a
+// channel, kStates states a lane, run the recurrence; then the threads finish and store the outputs. The next tile's
+// loads are in flight meanwhile.
+template <typename T, int kLanes, int kStates, int kTile>
+__global__ void __launch_bounds__(kScanThreads) scan_kernel(mmfree_cuda_ssm_args a, int blocks_per_group) {
+  constexpr int kChannels = kScanThreads / kLanes;           // channels of a CTA
+  constexpr int kRows = kScanThreads / kChannels;            // token rows that the threads cover at once
+  constexpr int kOwn = (kTile + kRows - 1) / kRows;          // tokens of a thread
+  constexpr int kN = kLanes * kStates;                       // states, padded
+  constexpr int kBC = (kTile * kN + kScanThreads - 1) / kScanThreads;  // elements of B (and of C) a thread stages
+  constexpr int kSteps = kLanes < 8 ? kLanes : 8;            // tokens summed over lanes together
+  static_assert(kTile % kSteps == 0 && kTile * kN * 8 + kTile * kChannels * 12 <= 48 * 1024, "tile shape");
+  __shared__ float2 s_in[kTile][kChannels];
+  __shared__ float s_y[kTile][kChannels];
+  __shared__ __align__(16) float s_b[kTile][kN], s_c[kTile][kN];
+
+  const int64_t seq = blockIdx.y;
+  int64_t b, e;
+  if (!sequence_rows(a.seq_starts, static_cast<int64_t>(a.tokens), seq, b, e) || b == e) return;
+  const int64_t slot = sequence_slot(a.slots, static_cast<int64_t>(a.slot_count), seq);
+  if (slot < 0) return;
+  const int tid = threadIdx.x, lane = tid % kLanes, states = static_cast<int>(a.states);
+  const int64_t channels = static_cast<int64_t>(a.channels), per_group = channels / static_cast<int64_t>(a.groups);
+  const int64_t group = blockIdx.x / blocks_per_group;
+  const int64_t first = (blockIdx.x - group * blocks_per_group) * kChannels;  // within the group
+  const int live = static_cast<int>(min(static_cast<int64_t>(kChannels), per_group - first));
+  const int64_t base = group * per_group + first;
+
+  // the channel this thread loads and stores, and the one whose states it holds
+  const int ch = tid % kChannels, row = tid / kChannels, sch = tid / kLanes;
+  const int64_t d = base + min(ch, live - 1), ds = base + min(sch, live - 1);
+  const float skip = a.D ? a.D[d] : 0.0f, bias = a.dt_bias ? a.dt_bias[d] : 0.0f;
+  const bool gate = a.z != nullptr, softplus = a.dt_softplus != 0;
+  const int64_t ldx = static_cast<int64_t>(a.ldx), ldt = static_cast<int64_t>(a.ld_dt), ldz = static_cast<int64_t>(a.ldz),
+                ldb = static_cast<int64_t>(a.ldb), ldc = static_cast<int64_t>(a.ldc), ldo = static_cast<int64_t>(a.ld_out);
+  const T* px = static_cast<const T*>(a.x) + d;
+  const T* pt = static_cast<const T*>(a.dt) + d;
+  const T* pz = gate ? static_cast<const T*>(a.z) + d : nullptr;
+  const T* pb = static_cast<const T*>(a.B) + group * states;
+  const T* pc = static_cast<const T*>(a.C) + group * states;
+  T* po = static_cast<T*>(a.out) + d;
+
+  float* state = a.state ? a.state + (slot * channels + ds) * states : nullptr;
+  f32x2 h[kStates / 2], rate[kStates / 2];
+#pragma unroll
+  for (int j = 0; j < kStates / 2; ++j) {
+    float hv[2], rv[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int n = lane * kStates + 2 * j + i;
+      hv[i] = n < states && state ? state[n] : 0.0f;
+      rv[i] = n < states ? a.A[ds * states + n] * kLog2E : 0.0f;
+    }
+    h[j] = pack2(hv[0], hv[1]);
+    rate[j] = pack2(rv[0], rv[1]);
+  }
+
+  T rx[kOwn], rt[kOwn], rz[kOwn], rb[kBC], rc[kBC];
+  const auto load = [&](int64_t t0) {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int64_t t = min(t0 + row + i * kRows, e - 1);
+      rx[i] = px[t * ldx];
+      rt[i] = pt[t * ldt];
+      if (gate) rz[i] = pz[t * ldz];
+    }
+#pragma unroll
+    for (int i = 0; i < kBC; ++i) {
+      const int at = tid + i * kScanThreads, n = min(at % kN, states - 1);
+      const int64_t t = min(t0 + at / kN, e - 1);
+      rb[i] = pb[t * ldb + n];
+      rc[i] = pc[t * ldc + n];
+    }
+  };
+  load(b);
+  for (int64_t t0 = b; t0 < e; t0 += kTile) {
+    const int left = static_cast<int>(min(static_cast<int64_t>(kTile), e - t0));
+    float x[kOwn], g[kOwn];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int t = row + i * kRows;
+      x[i] = to_f32(rx[i]);
+      float delta = to_f32(rt[i]) + bias;
+      if (softplus) delta = softplus_fast(delta);
+      // behind the sequence's end: a decay of 1 and no input
+      if (t < kTile) s_in[t][ch] = t < left ? make_float2(delta, delta * x[i]) : make_float2(0.0f, 0.0f);
+      g[i] = gate ? to_f32(rz[i]) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < kBC; ++i) {
+      const int at = tid + i * kScanThreads, n = at % kN;
+      if (kTile * kN % kScanThreads && at >= kTile * kN) break;
+      s_b[at / kN][n] = n < states ? to_f32(rb[i]) : 0.0f;
+      s_c[at / kN][n] = n < states ? to_f32(rc[i]) : 0.0f;
+    }
+    __syncthreads();
+    if (t0 + kTile < e) load(t0 + kTile);
+    for (int t = 0; t < kTile; t += kSteps) {
+      if (t >= left) break;
+      float y[kSteps];
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const float2 in = s_in[t + k][sch];
+        const f32x2 dd = pack2(in.x, in.x), dx = pack2(in.y, in.y);
+        f32x2 sum = pack2(0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < kStates / 2; ++j) {
+          const f32x2 bv = *reinterpret_cast<const f32x2*>(&s_b[t + k][lane * kStates + 2 * j]);
+          const f32x2 cv = *reinterpret_cast<const f32x2*>(&s_c[t + k][lane * kStates + 2 * j]);
+          float lo, hi;
+          unpack2(mul2(dd, rate[j]), lo, hi);
+          h[j] = fma2(pack2(ex2(lo), ex2(hi)), h[j], mul2(dx, bv));
+          sum = fma2(cv, h[j], sum);
+        }
+        float lo, hi;
+        unpack2(sum, lo, hi);
+        y[k] = lo + hi;
+      }
+      const float r = transpose_sum<kLanes, kSteps>(y, lane);
+      if (lane < kSteps) s_y[t + lane][sch] = r;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int t = row + i * kRows;
+      if (t >= left) break;
+      float y = fmaf(skip, x[i], s_y[t][ch]);
+      if (gate) y *= silu_fast(g[i]);
+      if (ch < live) po[(t0 + t) * ldo] = from_f32<T>(y);
+    }
+  }
+  if (state && sch < live) {
+#pragma unroll
+    for (int j = 0; j < kStates / 2; ++j) {
+      float hv[2];
+      unpack2(h[j], hv[0], hv[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (lane * kStates + 2 * j + i < states) state[lane * kStates + 2 * j + i] = hv[i];
+    }
+  }
+}
+
+template <typename T, int kLanes, int kStates, int kTile>
+cudaError_t scan_launch(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
+  constexpr int kChannels = kScanThreads / kLanes;
+  const int blocks = static_cast<int>(ceil_div(static_cast<int64_t>(a.channels / a.groups), kChannels));
+  // channel blocks fastest: consecutive CTAs go to different SMs, so every SM gets its share of each sequence
+  const dim3 grid(static_cast<unsigned>(blocks * a.groups), static_cast<unsigned>(a.seqs));
+  return launch_k(scan_kernel<T, kLanes, kStates, kTile>, grid, dim3(kScanThreads), 0, s, false, a, blocks);
+}
+
+// Lanes of a channel: four states a lane, eight where 32 lanes of four do not reach.
+template <typename T>
+cudaError_t scan_type(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
+  if (a.states <= 4) return scan_launch<T, 1, 4, 8>(a, s);
+  if (a.states <= 8) return scan_launch<T, 2, 4, 16>(a, s);
+  if (a.states <= 16) return scan_launch<T, 4, 4, 32>(a, s);
+  if (a.states <= 32) return scan_launch<T, 8, 4, 32>(a, s);
+  if (a.states <= 64) return scan_launch<T, 16, 4, 32>(a, s);
+  if (a.states <= 128) return scan_launch<T, 32, 4, 32>(a, s);
+  return scan_launch<T, 32, 8, 16>(a, s);
+}
+
+cudaError_t step_any(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
   int lanes = 1;
   while (lanes < 32 && lanes < static_cast<int>(a.states)) lanes *= 2;
   const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.channels) * lanes, 128)), static_cast<unsigned>(a.seqs));
   mark_device();
   switch (a.type) {
-    case MMFREE_T_F32: return launch_k(ssm_kernel<float>, grid, dim3(128), 0, s, false, a, lanes, step);
-    case MMFREE_T_BF16: return launch_k(ssm_kernel<__nv_bfloat16>, grid, dim3(128), 0, s, false, a, lanes, step);
-    default: return launch_k(ssm_kernel<__half>, grid, dim3(128), 0, s, false, a, lanes, step);
+    case MMFREE_T_F32: return launch_k(ssm_kernel<float>, grid, dim3(128), 0, s, false, a, lanes, true);
+    case MMFREE_T_BF16: return launch_k(ssm_kernel<__nv_bfloat16>, grid, dim3(128), 0, s, false, a, lanes, true);
+    default: return launch_k(ssm_kernel<__half>, grid, dim3(128), 0, s, false, a, lanes, true);
+  }
+}
+
+cudaError_t scan_any(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
+  mark_device();
+  switch (a.type) {
+    case MMFREE_T_F32: return scan_type<float>(a, s);
+    case MMFREE_T_BF16: return scan_type<__nv_bfloat16>(a, s);
+    default: return scan_type<__half>(a, s);
   }
 }
 
@@ -319,7 +568,7 @@ cudaError_t take_sequence_flags(cudaStream_t s, uint32_t* flags) {
 
 cudaError_t launch_causal_conv(const mmfree_cuda_conv_args& a, cudaStream_t s) { return conv_any(a, false, s); }
 cudaError_t launch_causal_conv_step(const mmfree_cuda_conv_args& a, cudaStream_t s) { return conv_any(a, true, s); }
-cudaError_t launch_selective_scan(const mmfree_cuda_ssm_args& a, int, cudaStream_t s) { return ssm_any(a, false, s); }
-cudaError_t launch_selective_step(const mmfree_cuda_ssm_args& a, cudaStream_t s) { return ssm_any(a, true, s); }
+cudaError_t launch_selective_scan(const mmfree_cuda_ssm_args& a, int, cudaStream_t s) { return scan_any(a, s); }
+cudaError_t launch_selective_step(const mmfree_cuda_ssm_args& a, cudaStream_t s) { return step_any(a, s); }
 
 }  // namespace mmfree_cuda
