@@ -363,40 +363,111 @@ __device__ __forceinline__ float transpose_sum(float (&v)[kSteps], int lane) {
   return r;
 }
 
-constexpr int kScanThreads = 128;
+constexpr int kScanThreads = 128;  // of each half of a CTA
 
-// One CTA: kScanThreads / kLanes channels of one group and one sequence, in tiles of kTile tokens. The threads first
-// turn the tile's x and dt into (delta, delta * x) in shared memory, once per token and channel; then kLanes lanes a
-// channel, kStates states a lane, run the recurrence; then the threads finish and store the outputs. The next tile's
-// loads are in flight meanwhile.
+// Shared memory of a scan CTA: what the two halves hand over, by tile.
+template <int kTile, int kChannels, int kN>
+struct ScanShared {
+  float2 in[2][kTile][kChannels];    // delta, delta * x
+  float2 finish[3][kTile][kChannels];  // D * x, silu(z)
+  float y[2][kTile][kChannels];
+  float b[2][kTile][kN], c[2][kTile][kN];
+};
+
+// One CTA: kScanThreads / kLanes channels of one group and one sequence, in tiles of kTile tokens, by two halves.
+// The first half runs the recurrence, kLanes lanes a channel and kStates states a lane. The second half meanwhile
+// turns the next tile's x, dt and z into what the recurrence and the outputs need, once per token and channel,
+// finishes and stores the previous tile's outputs, and has the tile after the next in flight. They meet at one
+// barrier a tile. In one half the two jobs alternated, and each left the issue slots of its latencies unused.
 template <typename T, int kLanes, int kStates, int kTile>
-__global__ void __launch_bounds__(kScanThreads) scan_kernel(mmfree_cuda_ssm_args a, int blocks_per_group) {
+__global__ void __launch_bounds__(2 * kScanThreads, 2) scan_kernel(mmfree_cuda_ssm_args a, int blocks_per_group) {
   constexpr int kChannels = kScanThreads / kLanes;           // channels of a CTA
-  constexpr int kRows = kScanThreads / kChannels;            // token rows that the threads cover at once
-  constexpr int kOwn = (kTile + kRows - 1) / kRows;          // tokens of a thread
+  constexpr int kRows = kScanThreads / kChannels;            // token rows that the second half covers at once
+  constexpr int kOwn = (kTile + kRows - 1) / kRows;          // tokens of one of its threads
   constexpr int kN = kLanes * kStates;                       // states, padded
-  constexpr int kBC = (kTile * kN + kScanThreads - 1) / kScanThreads;  // elements of B (and of C) a thread stages
+  constexpr int kBC = (kTile * kN + kScanThreads - 1) / kScanThreads;  // elements of B (and of C) it stages
   constexpr int kSteps = kLanes < 8 ? kLanes : 8;            // tokens summed over lanes together
-  static_assert(kTile % kSteps == 0 && kTile * kN * 8 + kTile * kChannels * 12 <= 48 * 1024, "tile shape");
-  __shared__ float2 s_in[kTile][kChannels];
-  __shared__ float s_y[kTile][kChannels];
-  __shared__ __align__(16) float s_b[kTile][kN], s_c[kTile][kN];
+  static_assert(kTile % kSteps == 0, "tile shape");
+  extern __shared__ __align__(16) char smem_raw[];
+  auto& sh = *reinterpret_cast<ScanShared<kTile, kChannels, kN>*>(smem_raw);
 
   const int64_t seq = blockIdx.y;
   int64_t b, e;
   if (!sequence_rows(a.seq_starts, static_cast<int64_t>(a.tokens), seq, b, e) || b == e) return;
   const int64_t slot = sequence_slot(a.slots, static_cast<int64_t>(a.slot_count), seq);
   if (slot < 0) return;
-  const int tid = threadIdx.x, lane = tid % kLanes, states = static_cast<int>(a.states);
+  const int tid = threadIdx.x % kScanThreads, states = static_cast<int>(a.states);
   const int64_t channels = static_cast<int64_t>(a.channels), per_group = channels / static_cast<int64_t>(a.groups);
   const int64_t group = blockIdx.x / blocks_per_group;
   const int64_t first = (blockIdx.x - group * blocks_per_group) * kChannels;  // within the group
   const int live = static_cast<int>(min(static_cast<int64_t>(kChannels), per_group - first));
   const int64_t base = group * per_group + first;
+  const int tiles = static_cast<int>((e - b + kTile - 1) / kTile);
 
-  // the channel this thread loads and stores, and the one whose states it holds
-  const int ch = tid % kChannels, row = tid / kChannels, sch = tid / kLanes;
-  const int64_t d = base + min(ch, live - 1), ds = base + min(sch, live - 1);
+  if (threadIdx.x < kScanThreads) {
+    // ---- the recurrence
+    const int lane = tid % kLanes, ch = tid / kLanes;
+    const int64_t d = base + min(ch, live - 1);
+    float* state = a.state ? a.state + (slot * channels + d) * states : nullptr;
+    f32x2 h[kStates / 2], rate[kStates / 2];
+#pragma unroll
+    for (int j = 0; j < kStates / 2; ++j) {
+      float hv[2], rv[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int n = lane * kStates + 2 * j + i;
+        hv[i] = n < states && state ? state[n] : 0.0f;
+        rv[i] = n < states ? a.A[d * states + n] * kLog2E : 0.0f;
+      }
+      h[j] = pack2(hv[0], hv[1]);
+      rate[j] = pack2(rv[0], rv[1]);
+    }
+    __syncthreads();
+    for (int tile = 0; tile < tiles; ++tile) {
+      const int buf = tile & 1;
+      const int left = static_cast<int>(min(static_cast<int64_t>(kTile), e - b - tile * kTile));
+      for (int t = 0; t < left; t += kSteps) {
+        float y[kSteps];
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          const float2 in = sh.in[buf][t + k][ch];
+          const f32x2 dd = pack2(in.x, in.x), dx = pack2(in.y, in.y);
+          f32x2 sum = pack2(0.0f, 0.0f);
+          f32x2 bv[kStates / 2], cv[kStates / 2];
+          *reinterpret_cast<Pack<float, kStates>*>(bv) = *reinterpret_cast<const Pack<float, kStates>*>(&sh.b[buf][t + k][lane * kStates]);
+          *reinterpret_cast<Pack<float, kStates>*>(cv) = *reinterpret_cast<const Pack<float, kStates>*>(&sh.c[buf][t + k][lane * kStates]);
+#pragma unroll
+          for (int j = 0; j < kStates / 2; ++j) {
+            float lo, hi;
+            unpack2(mul2(dd, rate[j]), lo, hi);
+            h[j] = fma2(pack2(ex2(lo), ex2(hi)), h[j], mul2(dx, bv[j]));
+            sum = fma2(cv[j], h[j], sum);
+          }
+          float lo, hi;
+          unpack2(sum, lo, hi);
+          y[k] = lo + hi;
+        }
+        const float r = transpose_sum<kLanes, kSteps>(y, lane);
+        if (lane < kSteps) sh.y[buf][t + lane][ch] = r;
+      }
+      __syncthreads();
+    }
+    if (state && ch < live) {
+#pragma unroll
+      for (int j = 0; j < kStates / 2; ++j) {
+        float hv[2];
+        unpack2(h[j], hv[0], hv[1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (lane * kStates + 2 * j + i < states) state[lane * kStates + 2 * j + i] = hv[i];
+      }
+    }
+    return;
+  }
+
+  // ---- loads, per-token work and outputs
+  const int ch = tid % kChannels, row = tid / kChannels;
+  const int64_t d = base + min(ch, live - 1);
   const float skip = a.D ? a.D[d] : 0.0f, bias = a.dt_bias ? a.dt_bias[d] : 0.0f;
   const bool gate = a.z != nullptr, softplus = a.dt_softplus != 0;
   const int64_t ldx = static_cast<int64_t>(a.ldx), ldt = static_cast<int64_t>(a.ld_dt), ldz = static_cast<int64_t>(a.ldz),
@@ -407,24 +478,9 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(mmfree_cuda_ssm_args
   const T* pb = static_cast<const T*>(a.B) + group * states;
   const T* pc = static_cast<const T*>(a.C) + group * states;
   T* po = static_cast<T*>(a.out) + d;
-
-  float* state = a.state ? a.state + (slot * channels + ds) * states : nullptr;
-  f32x2 h[kStates / 2], rate[kStates / 2];
-#pragma unroll
-  for (int j = 0; j < kStates / 2; ++j) {
-    float hv[2], rv[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int n = lane * kStates + 2 * j + i;
-      hv[i] = n < states && state ? state[n] : 0.0f;
-      rv[i] = n < states ? a.A[ds * states + n] * kLog2E : 0.0f;
-    }
-    h[j] = pack2(hv[0], hv[1]);
-    rate[j] = pack2(rv[0], rv[1]);
-  }
-
   T rx[kOwn], rt[kOwn], rz[kOwn], rb[kBC], rc[kBC];
-  const auto load = [&](int64_t t0) {
+  const auto load = [&](int tile) {
+    const int64_t t0 = b + tile * kTile;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int64_t t = min(t0 + row + i * kRows, e - 1);
@@ -440,82 +496,65 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(mmfree_cuda_ssm_args
       rc[i] = pc[t * ldc + n];
     }
   };
-  load(b);
-  for (int64_t t0 = b; t0 < e; t0 += kTile) {
-    const int left = static_cast<int>(min(static_cast<int64_t>(kTile), e - t0));
-    float x[kOwn], g[kOwn];
+  const auto prepare = [&](int tile) {
+    const int buf = tile & 1, fin = tile % 3;
+    const int64_t left = e - b - tile * kTile;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int t = row + i * kRows;
-      x[i] = to_f32(rx[i]);
+      if (kTile % kRows && t >= kTile) break;
+      const float x = to_f32(rx[i]);
       float delta = to_f32(rt[i]) + bias;
       if (softplus) delta = softplus_fast(delta);
       // behind the sequence's end: a decay of 1 and no input
-      if (t < kTile) s_in[t][ch] = t < left ? make_float2(delta, delta * x[i]) : make_float2(0.0f, 0.0f);
-      g[i] = gate ? to_f32(rz[i]) : 0.0f;
+      sh.in[buf][t][ch] = t < left ? make_float2(delta, delta * x) : make_float2(0.0f, 0.0f);
+      sh.finish[fin][t][ch] = make_float2(skip * x, gate ? silu_fast(to_f32(rz[i])) : 1.0f);
     }
 #pragma unroll
     for (int i = 0; i < kBC; ++i) {
       const int at = tid + i * kScanThreads, n = at % kN;
       if (kTile * kN % kScanThreads && at >= kTile * kN) break;
-      s_b[at / kN][n] = n < states ? to_f32(rb[i]) : 0.0f;
-      s_c[at / kN][n] = n < states ? to_f32(rc[i]) : 0.0f;
+      sh.b[buf][at / kN][n] = n < states ? to_f32(rb[i]) : 0.0f;
+      sh.c[buf][at / kN][n] = n < states ? to_f32(rc[i]) : 0.0f;
     }
-    __syncthreads();
-    if (t0 + kTile < e) load(t0 + kTile);
-    for (int t = 0; t < kTile; t += kSteps) {
-      if (t >= left) break;
-      float y[kSteps];
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        const float2 in = s_in[t + k][sch];
-        const f32x2 dd = pack2(in.x, in.x), dx = pack2(in.y, in.y);
-        f32x2 sum = pack2(0.0f, 0.0f);
-#pragma unroll
-        for (int j = 0; j < kStates / 2; ++j) {
-          const f32x2 bv = *reinterpret_cast<const f32x2*>(&s_b[t + k][lane * kStates + 2 * j]);
-          const f32x2 cv = *reinterpret_cast<const f32x2*>(&s_c[t + k][lane * kStates + 2 * j]);
-          float lo, hi;
-          unpack2(mul2(dd, rate[j]), lo, hi);
-          h[j] = fma2(pack2(ex2(lo), ex2(hi)), h[j], mul2(dx, bv));
-          sum = fma2(cv, h[j], sum);
-        }
-        float lo, hi;
-        unpack2(sum, lo, hi);
-        y[k] = lo + hi;
-      }
-      const float r = transpose_sum<kLanes, kSteps>(y, lane);
-      if (lane < kSteps) s_y[t + lane][sch] = r;
-    }
-    __syncthreads();
+  };
+  const auto finish = [&](int tile) {
+    const int buf = tile & 1, fin = tile % 3;
+    const int64_t t0 = b + tile * kTile, left = e - t0;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int t = row + i * kRows;
-      if (t >= left) break;
-      float y = fmaf(skip, x[i], s_y[t][ch]);
-      if (gate) y *= silu_fast(g[i]);
-      if (ch < live) po[(t0 + t) * ldo] = from_f32<T>(y);
+      if (t >= left || (kTile % kRows && t >= kTile)) break;
+      const float2 f = sh.finish[fin][t][ch];
+      if (ch < live) po[(t0 + t) * ldo] = from_f32<T>((sh.y[buf][t][ch] + f.x) * f.y);
     }
+  };
+  load(0);
+  prepare(0);
+  if (tiles > 1) load(1);
+  __syncthreads();
+  for (int tile = 0; tile < tiles; ++tile) {  // the first half is at `tile`
+    if (tile + 1 < tiles) prepare(tile + 1);
+    if (tile + 2 < tiles) load(tile + 2);
+    if (tile > 0) finish(tile - 1);
+    __syncthreads();
   }
-  if (state && sch < live) {
-#pragma unroll
-    for (int j = 0; j < kStates / 2; ++j) {
-      float hv[2];
-      unpack2(h[j], hv[0], hv[1]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (lane * kStates + 2 * j + i < states) state[lane * kStates + 2 * j + i] = hv[i];
-    }
-  }
+  finish(tiles - 1);
 }
 
 template <typename T, int kLanes, int kStates, int kTile>
 cudaError_t scan_launch(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
   constexpr int kChannels = kScanThreads / kLanes;
+  constexpr size_t kSmem = sizeof(ScanShared<kTile, kChannels, kLanes * kStates>);
   const int blocks = static_cast<int>(ceil_div(static_cast<int64_t>(a.channels / a.groups), kChannels));
   // channel blocks fastest: consecutive CTAs go to different SMs, so every SM gets its share of each sequence
   const dim3 grid(static_cast<unsigned>(blocks * a.groups), static_cast<unsigned>(a.seqs));
-  return launch_k(scan_kernel<T, kLanes, kStates, kTile>, grid, dim3(kScanThreads), 0, s, false, a, blocks);
+  if (kSmem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(scan_kernel<T, kLanes, kStates, kTile>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(kSmem));
+    if (e != cudaSuccess) return e;
+  }
+  return launch_k(scan_kernel<T, kLanes, kStates, kTile>, grid, dim3(2 * kScanThreads), kSmem, s, false, a, blocks);
 }
 
 // Lanes of a channel: four states a lane, eight where 32 lanes of four do not reach.
