@@ -5,6 +5,8 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <cstring>
+#include <type_traits>
 
 namespace mmfree_cuda {
 
@@ -25,6 +27,21 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <typename T, int V>
 struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
   T v[V];
+};
+
+// V elements as whole words, for values that stay in flight: a load into single 16-bit elements is taken apart, and so
+// waited for, where it is issued.
+template <typename T, int V>
+struct Words {
+  static constexpr int kBytes = sizeof(T) * V;
+  using Type = std::conditional_t<kBytes == 2, uint16_t, std::conditional_t<kBytes == 4, uint32_t, std::conditional_t<kBytes == 8, uint2, uint4>>>;
+  Type w;
+  __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const Type*>(p); }
+  __device__ __forceinline__ float operator[](int i) const {
+    Pack<T, V> k;
+    memcpy(&k, &w, kBytes);
+    return to_f32(k.v[i]);
+  }
 };
 
 // V elements from a 16-byte aligned address (kVec), or the first n of them one by one.

@@ -10,6 +10,7 @@
 #include "elements.cuh"
 
 #include <atomic>
+#include <type_traits>
 
 namespace mmfree_cuda {
 
@@ -363,210 +364,372 @@ __device__ __forceinline__ float transpose_sum(float (&v)[kSteps], int lane) {
   return r;
 }
 
-constexpr int kScanThreads = 128;  // of each half of a CTA
+// An asynchronous copy of 4, 8 or 16 bytes from global to shared memory.
+template <int kBytes>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(src), "n"(kBytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
 
-// Shared memory of a scan CTA: what the two halves hand over, by tile.
-template <int kTile, int kChannels, int kN>
-struct ScanShared {
-  float2 in[2][kTile][kChannels];    // delta, delta * x
-  float2 finish[3][kTile][kChannels];  // D * x, silu(z)
-  float y[2][kTile][kChannels];
-  float b[2][kTile][kN], c[2][kTile][kN];
+// The shape of a scan CTA. kLanes lanes hold the states of kPer neighbouring channels, kStates states of each a lane.
+template <typename T, int kLanes_, int kStates_, int kPer_, int kTile_, int kScan_, int kHelpers_, int kCtas_, int kBytes_>
+struct ScanShape {
+  using Type = T;
+  static constexpr int kLanes = kLanes_, kStates = kStates_, kPer = kPer_, kTile = kTile_;
+  static constexpr int kScan = kScan_;                          // threads of the recurrence
+  static constexpr int kHelpers = kHelpers_;                    // threads that load, prepare and store
+  static constexpr int kCtas = kCtas_;                          // CTAs an SM that the registers leave room for
+  static constexpr int kBytes = kBytes_;                        // of an access: 16 or 4, copied asynchronously, or 0: one element
+  static constexpr bool kVec = kBytes > 0;
+  static constexpr int kN = kLanes * kStates;                   // states, padded
+  static constexpr int kChannels = kScan / kLanes * kPer;
+  static constexpr int kWide = kVec ? kBytes / sizeof(T) : 1;
+  static constexpr int V = kWide < kChannels ? kWide : kChannels, VB = kWide < 4 ? kWide : 4;  // channels and states of one access
+  static constexpr int kColumns = kChannels / V;                // helper threads along a token
+  static constexpr int kRows = kHelpers / kColumns;             // tokens that the helpers cover at once
+  static constexpr int kOwn = (kTile + kRows - 1) / kRows;      // tokens of a helper
+  static constexpr int kBC = (kTile * kN / VB + kHelpers - 1) / kHelpers;  // vectors of B (and of C) of a helper
+  static constexpr int kStages = kVec ? 4 : 1;
+  struct Raw {  // one tile as it lies in memory; every helper reads what it copied itself
+    Pack<T, V> x[kOwn][kHelpers], dt[kOwn][kHelpers], z[kOwn][kHelpers];
+    Pack<T, VB> b[kBC][kHelpers], c[kBC][kHelpers];
+  };
+  struct Shared {
+    float2 in[2][kTile][kChannels];  // delta, delta * x
+    float y[2][kTile][kChannels];
+    float b[2][kTile][kN], c[2][kTile][kN];
+    Raw raw[kStages];
+  };
 };
 
-// One CTA: kScanThreads / kLanes channels of one group and one sequence, in tiles of kTile tokens, by two halves.
-// The first half runs the recurrence, kLanes lanes a channel and kStates states a lane. The second half meanwhile
-// turns the next tile's x, dt and z into what the recurrence and the outputs need, once per token and channel,
-// finishes and stores the previous tile's outputs, and has the tile after the next in flight. They meet at one
-// barrier a tile. In one half the two jobs alternated, and each left the issue slots of its latencies unused.
-template <typename T, int kLanes, int kStates, int kTile>
-__global__ void __launch_bounds__(2 * kScanThreads, 2) scan_kernel(mmfree_cuda_ssm_args a, int blocks_per_group) {
-  constexpr int kChannels = kScanThreads / kLanes;           // channels of a CTA
-  constexpr int kRows = kScanThreads / kChannels;            // token rows that the second half covers at once
-  constexpr int kOwn = (kTile + kRows - 1) / kRows;          // tokens of one of its threads
-  constexpr int kN = kLanes * kStates;                       // states, padded
-  constexpr int kBC = (kTile * kN + kScanThreads - 1) / kScanThreads;  // elements of B (and of C) it stages
-  constexpr int kSteps = kLanes < 8 ? kLanes : 8;            // tokens summed over lanes together
-  static_assert(kTile % kSteps == 0, "tile shape");
+// One CTA: a block of channels of one group and one sequence, in tiles of kTile tokens, by two halves. The first
+// runs the recurrence. The second, the helpers, meanwhile turns the next tile's x and dt into (delta, delta * x),
+// once per token and channel, finishes and stores the previous tile's outputs, and keeps two more tiles in flight
+// from memory. They meet at one barrier a tile. In one half the jobs alternated, and each left the issue slots of
+// its latencies unused.
+// What a turn of the recurrence reads from shared memory bounds it next to the special-function unit (128 bytes of
+// registers a clock): kPer channels a lane share one read of B and C.
+template <typename S>
+__global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(mmfree_cuda_ssm_args a, int blocks_per_group) {
+  using T = typename S::Type;
+  constexpr int kLanes = S::kLanes, kStates = S::kStates, kPer = S::kPer, kTile = S::kTile, kN = S::kN, V = S::V, VB = S::VB;
+  constexpr int kGroup = 4;                                  // tokens of a turn of the recurrence
+  constexpr int kSteps = kLanes < kGroup ? kLanes : kGroup;  // tokens summed over lanes together
+  constexpr int kPairs = kStates / 2;
+  static_assert(kTile % kGroup == 0 && sizeof(typename S::Shared) <= 227 * 1024, "tile shape");
   extern __shared__ __align__(16) char smem_raw[];
-  auto& sh = *reinterpret_cast<ScanShared<kTile, kChannels, kN>*>(smem_raw);
+  auto& sh = *reinterpret_cast<typename S::Shared*>(smem_raw);
 
   const int64_t seq = blockIdx.y;
   int64_t b, e;
   if (!sequence_rows(a.seq_starts, static_cast<int64_t>(a.tokens), seq, b, e) || b == e) return;
   const int64_t slot = sequence_slot(a.slots, static_cast<int64_t>(a.slot_count), seq);
   if (slot < 0) return;
-  const int tid = threadIdx.x % kScanThreads, states = static_cast<int>(a.states);
+  const int states = static_cast<int>(a.states);
   const int64_t channels = static_cast<int64_t>(a.channels), per_group = channels / static_cast<int64_t>(a.groups);
   const int64_t group = blockIdx.x / blocks_per_group;
-  const int64_t first = (blockIdx.x - group * blocks_per_group) * kChannels;  // within the group
-  const int live = static_cast<int>(min(static_cast<int64_t>(kChannels), per_group - first));
+  const int64_t first = (blockIdx.x - group * blocks_per_group) * S::kChannels;  // within the group
+  const int live = static_cast<int>(min(static_cast<int64_t>(S::kChannels), per_group - first));
   const int64_t base = group * per_group + first;
-  const int tiles = static_cast<int>((e - b + kTile - 1) / kTile);
+  const int length = static_cast<int>(e - b), tiles = (length + kTile - 1) / kTile;
 
-  if (threadIdx.x < kScanThreads) {
+  if (threadIdx.x < S::kScan) {
     // ---- the recurrence
-    const int lane = tid % kLanes, ch = tid / kLanes;
-    const int64_t d = base + min(ch, live - 1);
-    float* state = a.state ? a.state + (slot * channels + d) * states : nullptr;
-    f32x2 h[kStates / 2], rate[kStates / 2];
+    const int lane = threadIdx.x % kLanes, ch = threadIdx.x / kLanes * kPer;
+    float* const pool = a.state ? a.state + slot * channels * states : nullptr;
+    f32x2 h[kPer][kPairs], rate[kPer][kPairs];
 #pragma unroll
-    for (int j = 0; j < kStates / 2; ++j) {
-      float hv[2], rv[2];
+    for (int c = 0; c < kPer; ++c) {
+      const int64_t d = base + min(ch + c, live - 1);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int n = lane * kStates + 2 * j + i;
-        hv[i] = n < states && state ? state[n] : 0.0f;
-        rv[i] = n < states ? a.A[d * states + n] * kLog2E : 0.0f;
-      }
-      h[j] = pack2(hv[0], hv[1]);
-      rate[j] = pack2(rv[0], rv[1]);
-    }
-    __syncthreads();
-    for (int tile = 0; tile < tiles; ++tile) {
-      const int buf = tile & 1;
-      const int left = static_cast<int>(min(static_cast<int64_t>(kTile), e - b - tile * kTile));
-      for (int t = 0; t < left; t += kSteps) {
-        float y[kSteps];
+      for (int j = 0; j < kPairs; ++j) {
+        float hv[2], rv[2];
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          const float2 in = sh.in[buf][t + k][ch];
-          const f32x2 dd = pack2(in.x, in.x), dx = pack2(in.y, in.y);
-          f32x2 sum = pack2(0.0f, 0.0f);
-          f32x2 bv[kStates / 2], cv[kStates / 2];
-          *reinterpret_cast<Pack<float, kStates>*>(bv) = *reinterpret_cast<const Pack<float, kStates>*>(&sh.b[buf][t + k][lane * kStates]);
-          *reinterpret_cast<Pack<float, kStates>*>(cv) = *reinterpret_cast<const Pack<float, kStates>*>(&sh.c[buf][t + k][lane * kStates]);
-#pragma unroll
-          for (int j = 0; j < kStates / 2; ++j) {
-            float lo, hi;
-            unpack2(mul2(dd, rate[j]), lo, hi);
-            h[j] = fma2(pack2(ex2(lo), ex2(hi)), h[j], mul2(dx, bv[j]));
-            sum = fma2(cv[j], h[j], sum);
-          }
-          float lo, hi;
-          unpack2(sum, lo, hi);
-          y[k] = lo + hi;
+        for (int i = 0; i < 2; ++i) {
+          const int n = lane * kStates + 2 * j + i;
+          hv[i] = n < states && pool ? pool[d * states + n] : 0.0f;
+          rv[i] = n < states ? a.A[d * states + n] * kLog2E : 0.0f;
         }
-        const float r = transpose_sum<kLanes, kSteps>(y, lane);
-        if (lane < kSteps) sh.y[buf][t + lane][ch] = r;
+        h[c][j] = pack2(hv[0], hv[1]);
+        rate[c][j] = pack2(rv[0], rv[1]);
+      }
+    }
+    // the recurrence over `count` turns from token t0 of the tile; the outputs are stored behind the last one, since
+    // a store between them would keep the next turn's loads from shared memory behind it
+    const auto turns = [&](int buf, int t0, auto count) {
+      constexpr int kCount = decltype(count)::value;
+      float out[kCount][kPer][kGroup / kSteps];
+#pragma unroll
+      for (int turn = 0; turn < kCount; ++turn) {
+        float y[kPer][kGroup];
+#pragma unroll
+        for (int k = 0; k < kGroup; ++k) {
+          const int t = t0 + turn * kGroup + k;
+          const Pack<float, 2 * kPer> in = *reinterpret_cast<const Pack<float, 2 * kPer>*>(&sh.in[buf][t][ch]);
+          f32x2 bv[kPairs], cv[kPairs];
+          *reinterpret_cast<Pack<float, kStates>*>(bv) = *reinterpret_cast<const Pack<float, kStates>*>(&sh.b[buf][t][lane * kStates]);
+          *reinterpret_cast<Pack<float, kStates>*>(cv) = *reinterpret_cast<const Pack<float, kStates>*>(&sh.c[buf][t][lane * kStates]);
+#pragma unroll
+          for (int c = 0; c < kPer; ++c) {
+            const f32x2 dl = pack2(in.v[2 * c], in.v[2 * c]), dx = pack2(in.v[2 * c + 1], in.v[2 * c + 1]);
+            f32x2 sum;
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) {
+              float lo, hi;
+              unpack2(mul2(dl, rate[c][j]), lo, hi);
+              h[c][j] = fma2(pack2(ex2(lo), ex2(hi)), h[c][j], mul2(dx, bv[j]));
+              sum = j ? fma2(cv[j], h[c][j], sum) : mul2(cv[j], h[c][j]);
+            }
+            float lo, hi;
+            unpack2(sum, lo, hi);
+            y[c][k] = lo + hi;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < kPer; ++c)
+#pragma unroll
+          for (int g = 0; g < kGroup; g += kSteps) {
+            float part[kSteps];
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) part[k] = y[c][g + k];
+            out[turn][c][g / kSteps] = transpose_sum<kLanes, kSteps>(part, lane);
+          }
+      }
+      if (lane < kSteps)
+#pragma unroll
+        for (int turn = 0; turn < kCount; ++turn)
+#pragma unroll
+          for (int g = 0; g < kGroup; g += kSteps) {
+            Pack<float, kPer> v;
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) v.v[c] = out[turn][c][g / kSteps];
+            *reinterpret_cast<Pack<float, kPer>*>(&sh.y[buf][t0 + turn * kGroup + g + lane][ch]) = v;
+          }
+    };
+    __syncthreads();
+    constexpr int kTurns = kTile / kGroup;
+    for (int tile = 0; tile < tiles; ++tile) {
+      const int buf = tile & 1, left = min(kTile, length - tile * kTile);
+      if (left > kTile - kGroup) {  // unrolled as a whole, so that loads and exponentials run ahead of the sums
+        turns(buf, 0, std::integral_constant<int, kTurns>{});
+      } else {
+#pragma unroll 1
+        for (int t = 0; t < left; t += 2 * kGroup) turns(buf, t, std::integral_constant<int, 2>{});
       }
       __syncthreads();
     }
-    if (state && ch < live) {
 #pragma unroll
-      for (int j = 0; j < kStates / 2; ++j) {
+    for (int c = 0; c < kPer; ++c) {
+      if (!pool || ch + c >= live) break;
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
         float hv[2];
-        unpack2(h[j], hv[0], hv[1]);
+        unpack2(h[c][j], hv[0], hv[1]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (lane * kStates + 2 * j + i < states) state[lane * kStates + 2 * j + i] = hv[i];
+        for (int i = 0; i < 2; ++i) {
+          const int n = lane * kStates + 2 * j + i;
+          if (n < states) pool[(base + ch + c) * states + n] = hv[i];
+        }
       }
     }
     return;
   }
 
-  // ---- loads, per-token work and outputs
-  const int ch = tid % kChannels, row = tid / kChannels;
-  const int64_t d = base + min(ch, live - 1);
-  const float skip = a.D ? a.D[d] : 0.0f, bias = a.dt_bias ? a.dt_bias[d] : 0.0f;
+  // ---- the helpers
+  constexpr int kOwn = S::kOwn, kRows = S::kRows, kBC = S::kBC, kHelpers = S::kHelpers;
+  const int tid = threadIdx.x - S::kScan, ch = tid % S::kColumns * V, row = tid / S::kColumns;
+  const bool mine = ch < live;  // whole vectors
+  const int64_t d = base + (mine ? ch : 0);
+  float skip[V], bias[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    skip[v] = a.D ? a.D[d + v] : 0.0f;
+    bias[v] = a.dt_bias ? a.dt_bias[d + v] : 0.0f;
+  }
   const bool gate = a.z != nullptr, softplus = a.dt_softplus != 0;
   const int64_t ldx = static_cast<int64_t>(a.ldx), ldt = static_cast<int64_t>(a.ld_dt), ldz = static_cast<int64_t>(a.ldz),
                 ldb = static_cast<int64_t>(a.ldb), ldc = static_cast<int64_t>(a.ldc), ldo = static_cast<int64_t>(a.ld_out);
-  const T* px = static_cast<const T*>(a.x) + d;
-  const T* pt = static_cast<const T*>(a.dt) + d;
-  const T* pz = gate ? static_cast<const T*>(a.z) + d : nullptr;
-  const T* pb = static_cast<const T*>(a.B) + group * states;
-  const T* pc = static_cast<const T*>(a.C) + group * states;
-  T* po = static_cast<T*>(a.out) + d;
-  T rx[kOwn], rt[kOwn], rz[kOwn], rb[kBC], rc[kBC];
+  const T* px = static_cast<const T*>(a.x) + b * ldx + d;
+  const T* pt = static_cast<const T*>(a.dt) + b * ldt + d;
+  const T* pz = gate ? static_cast<const T*>(a.z) + b * ldz + d : nullptr;
+  const T* pb = static_cast<const T*>(a.B) + group * states + b * ldb;
+  const T* pc = static_cast<const T*>(a.C) + group * states + b * ldc;
+  T* po = static_cast<T*>(a.out) + b * ldo + d;
   const auto load = [&](int tile) {
-    const int64_t t0 = b + tile * kTile;
+    if (tile < tiles) {
+      auto& raw = sh.raw[tile % S::kStages];
+      const int t0 = tile * kTile, most = length - 1 - t0;  // tokens behind the end read the last one again
+      const auto fetch = [](auto* dst, const T* src) {
+        if constexpr (S::kVec) copy_async<sizeof(*dst)>(dst, src);
+        else dst->v[0] = *src;
+      };
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-      const int64_t t = min(t0 + row + i * kRows, e - 1);
-      rx[i] = px[t * ldx];
-      rt[i] = pt[t * ldt];
-      if (gate) rz[i] = pz[t * ldz];
-    }
+      for (int i = 0; i < kOwn; ++i) {
+        if (kTile % kRows && row + i * kRows >= kTile) break;
+        const int64_t t = t0 + min(row + i * kRows, most);
+        fetch(&raw.x[i][tid], px + t * ldx);
+        fetch(&raw.dt[i][tid], pt + t * ldt);
+        if (gate) fetch(&raw.z[i][tid], pz + t * ldz);
+      }
 #pragma unroll
-    for (int i = 0; i < kBC; ++i) {
-      const int at = tid + i * kScanThreads, n = min(at % kN, states - 1);
-      const int64_t t = min(t0 + at / kN, e - 1);
-      rb[i] = pb[t * ldb + n];
-      rc[i] = pc[t * ldc + n];
+      for (int i = 0; i < kBC; ++i) {
+        const int at = (tid + i * kHelpers) * VB, n = min(at % kN, states - VB);
+        if (kTile * kN / VB % kHelpers && at >= kTile * kN) break;
+        const int64_t t = t0 + min(at / kN, most);
+        fetch(&raw.b[i][tid], pb + t * ldb + n);
+        fetch(&raw.c[i][tid], pc + t * ldc + n);
+      }
     }
+    if constexpr (S::kVec) copy_commit();
   };
   const auto prepare = [&](int tile) {
-    const int buf = tile & 1, fin = tile % 3;
-    const int64_t left = e - b - tile * kTile;
+    if (tile >= tiles) return;
+    const int buf = tile & 1, left = length - tile * kTile;
+    const auto& raw = sh.raw[tile % S::kStages];
+    // branches around whole arrays: around single elements they would keep the elements' chains one after another
+    float delta[kOwn][V], x[kOwn][V];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      if (kTile % kRows && row + i * kRows >= kTile) break;
+      const Pack<T, V> rx = raw.x[i][tid], rt = raw.dt[i][tid];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        x[i][v] = to_f32(rx.v[v]);
+        delta[i][v] = to_f32(rt.v[v]) + bias[v];
+      }
+    }
+    if (softplus) {
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v) delta[i][v] = softplus_fast(delta[i][v]);
+    }
+    if (left < kTile) {  // behind the sequence's end: a decay of 1 and no input, also where x is not finite
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (row + i * kRows >= left) delta[i][v] = x[i][v] = 0.0f;
+    }
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int t = row + i * kRows;
       if (kTile % kRows && t >= kTile) break;
-      const float x = to_f32(rx[i]);
-      float delta = to_f32(rt[i]) + bias;
-      if (softplus) delta = softplus_fast(delta);
-      // behind the sequence's end: a decay of 1 and no input
-      sh.in[buf][t][ch] = t < left ? make_float2(delta, delta * x) : make_float2(0.0f, 0.0f);
-      sh.finish[fin][t][ch] = make_float2(skip * x, gate ? silu_fast(to_f32(rz[i])) : 1.0f);
+      Pack<float, 2 * V> in;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        in.v[2 * v] = delta[i][v];
+        in.v[2 * v + 1] = delta[i][v] * x[i][v];
+      }
+      *reinterpret_cast<Pack<float, 2 * V>*>(&sh.in[buf][t][ch]) = in;
     }
 #pragma unroll
     for (int i = 0; i < kBC; ++i) {
-      const int at = tid + i * kScanThreads, n = at % kN;
-      if (kTile * kN % kScanThreads && at >= kTile * kN) break;
-      sh.b[buf][at / kN][n] = n < states ? to_f32(rb[i]) : 0.0f;
-      sh.c[buf][at / kN][n] = n < states ? to_f32(rc[i]) : 0.0f;
+      const int at = (tid + i * kHelpers) * VB, n = at % kN;
+      if (kTile * kN / VB % kHelpers && at >= kTile * kN) break;
+      const Pack<T, VB> rb = raw.b[i][tid], rc = raw.c[i][tid];
+      Pack<float, VB> vb, vc;
+#pragma unroll
+      for (int v = 0; v < VB; ++v) {
+        vb.v[v] = n < states ? to_f32(rb.v[v]) : 0.0f;
+        vc.v[v] = n < states ? to_f32(rc.v[v]) : 0.0f;
+      }
+      *reinterpret_cast<Pack<float, VB>*>(&sh.b[buf][at / kN][n]) = vb;
+      *reinterpret_cast<Pack<float, VB>*>(&sh.c[buf][at / kN][n]) = vc;
     }
   };
   const auto finish = [&](int tile) {
-    const int buf = tile & 1, fin = tile % 3;
-    const int64_t t0 = b + tile * kTile, left = e - t0;
+    const int buf = tile & 1, t0 = tile * kTile, left = length - t0;
+    const auto& raw = sh.raw[tile % S::kStages];
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int t = row + i * kRows;
-      if (t >= left || (kTile % kRows && t >= kTile)) break;
-      const float2 f = sh.finish[fin][t][ch];
-      if (ch < live) po[(t0 + t) * ldo] = from_f32<T>((sh.y[buf][t][ch] + f.x) * f.y);
+      if ((kTile % kRows && t >= kTile) || t >= left) break;
+      Pack<T, V> rx, rz;
+      if constexpr (S::kVec) {
+        rx = raw.x[i][tid];
+        if (gate) rz = raw.z[i][tid];
+      } else {
+        rx.v[0] = px[(t0 + t) * ldx];
+        if (gate) rz.v[0] = pz[(t0 + t) * ldz];
+      }
+      const Pack<float, V> p = *reinterpret_cast<const Pack<float, V>*>(&sh.y[buf][t][ch]);
+      float y[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) y[v] = fmaf(skip[v], to_f32(rx.v[v]), p.v[v]);
+      if (gate)
+#pragma unroll
+        for (int v = 0; v < V; ++v) y[v] *= silu_fast(to_f32(rz.v[v]));
+      if (mine) store_row<S::kVec>(po + static_cast<int64_t>(t0 + t) * ldo, V, y);
     }
   };
+  // before the first half's tile 0: tile 0 prepared; in its tile t: t + 1 prepared, t - 1 finished, then its stage filled
+  constexpr int kAhead = S::kStages - 1;
   load(0);
+  if constexpr (S::kVec) {
+    load(1);
+    load(2);
+    copy_wait<kAhead - 1>();
+  }
   prepare(0);
-  if (tiles > 1) load(1);
   __syncthreads();
-  for (int tile = 0; tile < tiles; ++tile) {  // the first half is at `tile`
-    if (tile + 1 < tiles) prepare(tile + 1);
-    if (tile + 2 < tiles) load(tile + 2);
+  for (int tile = 0; tile < tiles; ++tile) {
+    if constexpr (S::kVec) copy_wait<kAhead - 2>();
+    else load(tile + 1);
+    prepare(tile + 1);
     if (tile > 0) finish(tile - 1);
+    if constexpr (S::kVec) load(tile + kAhead);
     __syncthreads();
   }
   finish(tiles - 1);
 }
 
-template <typename T, int kLanes, int kStates, int kTile>
+template <typename S>
 cudaError_t scan_launch(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
-  constexpr int kChannels = kScanThreads / kLanes;
-  constexpr size_t kSmem = sizeof(ScanShared<kTile, kChannels, kLanes * kStates>);
-  const int blocks = static_cast<int>(ceil_div(static_cast<int64_t>(a.channels / a.groups), kChannels));
+  constexpr size_t kSmem = sizeof(typename S::Shared);
+  const int blocks = static_cast<int>(ceil_div(static_cast<int64_t>(a.channels / a.groups), S::kChannels));
   // channel blocks fastest: consecutive CTAs go to different SMs, so every SM gets its share of each sequence
   const dim3 grid(static_cast<unsigned>(blocks * a.groups), static_cast<unsigned>(a.seqs));
   if (kSmem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(scan_kernel<T, kLanes, kStates, kTile>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(kSmem));
+    const cudaError_t e = cudaFuncSetAttribute(scan_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
     if (e != cudaSuccess) return e;
   }
-  return launch_k(scan_kernel<T, kLanes, kStates, kTile>, grid, dim3(2 * kScanThreads), kSmem, s, false, a, blocks);
+  return launch_k(scan_kernel<S>, grid, dim3(S::kScan + S::kHelpers), kSmem, s, false, a, blocks);
 }
 
-// Lanes of a channel: four states a lane, eight where 32 lanes of four do not reach.
+template <typename T, int kBytes>
+cudaError_t scan_states(const mmfree_cuda_ssm_args& a, int sms, cudaStream_t s) {
+  if (a.states <= 4) return scan_launch<ScanShape<T, 1, 4, 1, 8, 128, 128, 2, kBytes>>(a, s);
+  if (a.states <= 8) return scan_launch<ScanShape<T, 2, 4, 1, 16, 128, 128, 2, kBytes>>(a, s);
+  if (a.states <= 16) {
+    // Two channels a lane (half the reads of B and C) where CTAs of 32 channels are several an SM, else one, on
+    // twice the warps: 16384 tokens in 8 sequences x 5120 channels take 658 against 668 us, one sequence of 4099
+    // x 4096 (one CTA an SM) 260 against 162 us.
+    if (static_cast<int64_t>(a.channels * a.seqs) >= 32 * 3 * static_cast<int64_t>(sms))
+      return scan_launch<ScanShape<T, 4, 4, 2, 16, 64, 64, 4, kBytes>>(a, s);
+    return scan_launch<ScanShape<T, 4, 4, 1, 32, 128, 128, 2, kBytes>>(a, s);
+  }
+  if (a.states <= 32) return scan_launch<ScanShape<T, 8, 4, 1, 32, 128, 128, 2, kBytes>>(a, s);
+  if (a.states <= 64) return scan_launch<ScanShape<T, 16, 4, 1, 32, 128, 128, 2, kBytes>>(a, s);
+  if (a.states <= 128) return scan_launch<ScanShape<T, 32, 4, 2, 16, 128, 128, 2, kBytes>>(a, s);
+  return scan_launch<ScanShape<T, 32, 8, 1, 8, 128, 128, 2, kBytes>>(a, s);
+}
+
 template <typename T>
-cudaError_t scan_type(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
-  if (a.states <= 4) return scan_launch<T, 1, 4, 8>(a, s);
-  if (a.states <= 8) return scan_launch<T, 2, 4, 16>(a, s);
-  if (a.states <= 16) return scan_launch<T, 4, 4, 32>(a, s);
-  if (a.states <= 32) return scan_launch<T, 8, 4, 32>(a, s);
-  if (a.states <= 64) return scan_launch<T, 16, 4, 32>(a, s);
-  if (a.states <= 128) return scan_launch<T, 32, 4, 32>(a, s);
-  return scan_launch<T, 32, 8, 16>(a, s);
+cudaError_t scan_type(const mmfree_cuda_ssm_args& a, int sms, cudaStream_t s) {
+  // whether x, dt, z and out can be accessed by `n` channels, and B and C by up to four states
+  const auto fits = [&](size_t n) {
+    const size_t m = n < 4 ? n : 4;
+    const auto one = [](const void* p, size_t pitch, size_t k) { return reinterpret_cast<uintptr_t>(p) % (k * sizeof(T)) == 0 && pitch % k == 0; };
+    return a.channels / a.groups % n == 0 && a.states % m == 0 && one(a.x, a.ldx, n) && one(a.dt, a.ld_dt, n) && one(a.z, a.ldz, n) &&
+           one(a.out, a.ld_out, n) && one(a.B, a.ldb, m) && one(a.C, a.ldc, m);
+  };
+  if (fits(16 / sizeof(T))) return scan_states<T, 16>(a, sms, s);
+  return fits(4 / sizeof(T)) ? scan_states<T, 4>(a, sms, s) : scan_states<T, 0>(a, sms, s);
 }
 
 cudaError_t step_any(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
@@ -581,12 +744,12 @@ cudaError_t step_any(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
   }
 }
 
-cudaError_t scan_any(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
+cudaError_t scan_any(const mmfree_cuda_ssm_args& a, int sms, cudaStream_t s) {
   mark_device();
   switch (a.type) {
-    case MMFREE_T_F32: return scan_type<float>(a, s);
-    case MMFREE_T_BF16: return scan_type<__nv_bfloat16>(a, s);
-    default: return scan_type<__half>(a, s);
+    case MMFREE_T_F32: return scan_type<float>(a, sms, s);
+    case MMFREE_T_BF16: return scan_type<__nv_bfloat16>(a, sms, s);
+    default: return scan_type<__half>(a, sms, s);
   }
 }
 
@@ -607,7 +770,7 @@ cudaError_t take_sequence_flags(cudaStream_t s, uint32_t* flags) {
 
 cudaError_t launch_causal_conv(const mmfree_cuda_conv_args& a, cudaStream_t s) { return conv_any(a, false, s); }
 cudaError_t launch_causal_conv_step(const mmfree_cuda_conv_args& a, cudaStream_t s) { return conv_any(a, true, s); }
-cudaError_t launch_selective_scan(const mmfree_cuda_ssm_args& a, int, cudaStream_t s) { return scan_any(a, s); }
+cudaError_t launch_selective_scan(const mmfree_cuda_ssm_args& a, int sm_count, cudaStream_t s) { return scan_any(a, sm_count, s); }
 cudaError_t launch_selective_step(const mmfree_cuda_ssm_args& a, cudaStream_t s) { return step_any(a, s); }
 
 }  // namespace mmfree_cuda
