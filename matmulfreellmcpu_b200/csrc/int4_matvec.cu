@@ -13,8 +13,10 @@
 // exact, summed in fp32, and a group's sum is scaled once.
 //
 // The order of a product's columns is free as long as weights and activations agree, so a lane
-// takes runs of consecutive columns of its weight row: 16-byte loads straight from the row-major
-// codes, no repacked copy of the weights.
+// takes 8 consecutive columns of its weight row, one word of the row-major codes: no repacked
+// copy of the weights. The words come through shared memory, filled by asynchronous copies two
+// turns ahead; rolled loops over it keep the code small (with the words in registers the
+// unrolled loops were bound by instruction fetches: 22 instead of KERNEL_US us for 2048 -> 32000).
 #include "block_ops.h"
 #include "common.cuh"
 #include "elements.cuh"
@@ -28,6 +30,7 @@ namespace {
 
 constexpr int kWarps = 8;       // of a CTA: they share its weight rows and split the columns
 constexpr int kTileK = 256;     // columns of a warp's turn (128 bytes of a weight row)
+constexpr int kTurnRuns = kTileK / 32;  // runs: 32 columns, 8 of each of the 4 lanes that share a row
 constexpr int kPitch = 36;      // words of a partial-sum row of 32 outputs: keeps its writers on different banks
 
 __device__ __forceinline__ float scale_value(const void* p, int type, int64_t i) {
@@ -72,10 +75,10 @@ struct RowType {
 };
 
 // Eight elements of a row from column k, `left` of them inside it (the others are 0).
-template <int kType, bool kVec>
-__device__ __forceinline__ void load_x(const char* row, int k, int left, uint32_t (&w)[RowType<kType>::kWords]) {
+template <int kType>
+__device__ __forceinline__ void load_x(const char* row, int k, int left, bool vec, uint32_t (&w)[RowType<kType>::kWords]) {
   constexpr int kBytes = RowType<kType>::kBytes, kWords = RowType<kType>::kWords;
-  if (kVec && left >= 8) {
+  if (vec && left >= 8) {
     const char* p = row + static_cast<int64_t>(k) * kBytes;
     if constexpr (kWords == 2) {
       const uint2 v = *reinterpret_cast<const uint2*>(p);
@@ -164,141 +167,168 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// kRun consecutive columns of a weight row from column k.
-template <int kRun, bool kVec>
-__device__ __forceinline__ void load_codes(const uint8_t* row, int k, int K, uint32_t (&w)[kRun / 8]) {
-  const uint8_t* p = row + k / 2;
-  if (kVec && k + kRun <= K) {
-    if constexpr (kRun == 32) {
-      const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
-      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    } else if constexpr (kRun == 16) {
-      const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
-      w[0] = v.x, w[1] = v.y;
-    } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
-    return;
-  }
-  const int bytes = (K - k + 1) / 2;  // left in the row
-#pragma unroll
-  for (int i = 0; i < kRun / 8; ++i) {
-    w[i] = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (4 * i + j < bytes) w[i] |= static_cast<uint32_t>(p[4 * i + j]) << (8 * j);
-  }
+// 16 bytes of which the first `bytes` are read and the others become 0.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 
-// A CTA: kBlocks blocks of 16 weight rows and 8 * kTiles activation rows at a time; its warps (and those of the other
-// CTAs of its cluster) split the columns into turns of kTileK. kRun: consecutive columns of a lane, so that the 4
-// lanes of a row cover 4 * kRun columns of ONE group: 32 (16-byte loads) where the group is a multiple of 128
-// columns, 16 for 64, else 8. The row blocks are walked by a fixed grid, the next turn's weights loaded while this
-// one's are multiplied.
-template <int kType, int kTiles, int kRun, bool kVec>
-__global__ void __launch_bounds__(32 * kWarps, kTiles == 4 ? 1 : 2) int4_kernel(Int4Args a, int splits, int m0) {
+template <int kTiles, bool kAligned>
+struct Int4Shape {
+  static constexpr int kBlocks = 2, kRows = 16 * kBlocks;  // weight rows of a CTA at a time
+  static constexpr int kCols = 8 * kTiles;                 // activation rows
+  static constexpr int kChunks = kAligned ? 8 : 9;         // 16-byte chunks of a row and turn
+  static constexpr int kCtas = kTiles == 4 ? 1 : 2;        // an SM
+  static constexpr int kStages = kTiles == 4 ? 3 : 2;
+  struct Warp {
+    uint4 codes[kStages][kRows][kChunks];
+    float scale[kTurnRuns][kRows];
+    uint32_t zero[kTurnRuns][kRows];
+  };
+  struct Shared {
+    Warp warp[kWarps];
+    float part[kWarps][kCols][kPitch];
+  };
+};
+
+// A CTA: 32 weight rows and 8 * kTiles activation rows at a time; its warps (and those of the other CTAs of its
+// cluster) split the columns into turns of kTileK. The row blocks are walked by a fixed grid.
+// kAligned: the rows of the codes start at multiples of 16 bytes. Otherwise the aligned chunks that a row's turn
+// touches are copied (a chunk with a byte of the row in it can be read as a whole) and its words put together from
+// two, shifted by the row's own offset.
+template <int kType, int kTiles, bool kAligned>
+__global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCtas) int4_kernel(Int4Args a, int splits, int m0, bool xvec) {
   using X = RowType<kType>;
-  constexpr int kBlocks = 2, kRows = 16 * kBlocks, kCols = 8 * kTiles, kRuns = kTileK / (4 * kRun), kWordsRun = kRun / 8;
-  constexpr int kBuffers = kTiles == 4 ? 1 : 2;  // two save a barrier a block where they fit
-  __shared__ float s_part[kBuffers][kWarps][kCols][kPitch];
+  using S = Int4Shape<kTiles, kAligned>;
+  constexpr int kBlocks = S::kBlocks, kRows = S::kRows, kCols = S::kCols, kChunks = S::kChunks, kStages = S::kStages;
+  extern __shared__ __align__(16) char smem_raw[];
+  auto& sh = *reinterpret_cast<typename S::Shared*>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int rank = blockIdx.x % splits;
-  const int K = a.K, turns = (K + kTileK - 1) / kTileK, blocks = (a.N + kRows - 1) / kRows;
+  auto& mine = sh.warp[warp];
+  const int rank = blockIdx.x % splits, step = gridDim.x / splits;
+  const int K = a.K, turns = (K + kTileK - 1) / kTileK, blocks = (a.N + kRows - 1) / kRows, bytes = (K + 1) / 2;
   const int stride = kWarps * splits, first = rank * kWarps + warp;
   const int live = min(kCols, a.M - m0);
-  // the activation row of this lane's operand in each tile (rows behind the last are not read)
-  const char* xrow[kTiles];
-#pragma unroll
-  for (int i = 0; i < kTiles; ++i) xrow[i] = static_cast<const char*>(a.x) + (m0 + 8 * i + g) * a.ldx * X::kBytes;
+  const char* const x = static_cast<const char*>(a.x) + static_cast<int64_t>(m0) * a.ldx * X::kBytes;
 
-  uint32_t w[kBlocks][2][kRuns][kWordsRun];
-  const auto fetch = [&](int block, int turn) {
-    if (block >= blocks || turn >= turns) return;
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int n = min(block * kRows + 16 * b + 8 * h + g, a.N - 1);
-#pragma unroll
-        for (int r = 0; r < kRuns; ++r) {
-          const int k = turn * kTileK + r * 4 * kRun + t * kRun;
-          if (k < K) {
-            load_codes<kRun, kVec>(a.codes + n * a.ldw, k, K, w[b][h][r]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < kWordsRun; ++i) w[b][h][r][i] = 0;
-          }
+  // the next turn to copy
+  int copy_block = blockIdx.x / splits, copy_turn = first, copied = 0;
+  const auto copy = [&] {
+    if (copy_block < blocks && first < turns) {
+      const uint32_t to = smem_u32(&mine.codes[copied % kStages][0][0]);
+      const int from = copy_turn * (kTileK / 2);
+      for (int i = lane; i < kRows * kChunks; i += 32) {
+        const int row = i / kChunks, c = i % kChunks;
+        const uint8_t* const line = a.codes + min(copy_block * kRows + row, a.N - 1) * a.ldw;
+        if constexpr (kAligned) {
+          const int at = from + 16 * c, left = min(max(bytes - at, 0), 16);
+          // chunks of a row are rotated by the row, so that 8 rows' words of one column are on different banks
+          copy16(to + (row * kChunks + (c ^ (row & 7))) * 16, left ? line + at : line, left);
+        } else {
+          const uint8_t* const at = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(line + from) & ~uintptr_t(15)) + 16 * c;
+          const bool any = at < line + bytes;
+          copy16(to + i * 16, any ? at : reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(line) & ~uintptr_t(15)), any ? 16 : 0);
         }
       }
+      if ((copy_turn += stride) >= turns) copy_turn = first, copy_block += step;
+    }
+    ++copied;
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  const int step = gridDim.x / splits;
-  int buf = 0;
-  fetch(blockIdx.x / splits, first);
-  for (int block = blockIdx.x / splits; block < blocks; block += step, buf = (buf + 1) % kBuffers) {
+  // scales and zero points of a turn: lane r has row r's, up to 8 groups
+  float next_scale[kTurnRuns];
+  uint32_t next_zero[kTurnRuns];
+  const auto fetch = [&](int block, int turn) {
+    const int64_t at = static_cast<int64_t>(min(block * kRows + lane, a.N - 1)) * a.parts;
+    const int g0 = turn * kTileK / a.group, g1 = min(a.parts - 1, (turn * kTileK + kTileK - 1) / a.group);
+#pragma unroll
+    for (int i = 0; i < kTurnRuns; ++i) {
+      if (g0 + i > g1) break;
+      next_scale[i] = scale_value(a.scales, a.scale_type, at + g0 + i);
+      next_zero[i] = a.zeros ? a.zeros[at + g0 + i] : 8u;
+    }
+  };
+  const auto keep = [&] {
+#pragma unroll
+    for (int i = 0; i < kTurnRuns; ++i) {
+      mine.scale[i][lane] = next_scale[i];
+      // 128 + z or 1024 + z twice (z up to 127 is exact)
+      uint32_t v;
+      if constexpr (X::kBf16) v = __bfloat16_as_ushort(__float2bfloat16_rn(128.0f + static_cast<float>(next_zero[i])));
+      else v = __half_as_ushort(__float2half_rn(1024.0f + static_cast<float>(next_zero[i])));
+      mine.zero[i][lane] = v | v << 16;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kTurnRuns; ++i) next_scale[i] = 0.0f, next_zero[i] = 0;
+#pragma unroll
+  for (int i = 0; i + 1 < kStages; ++i) copy();
+  if (blockIdx.x / splits < blocks && first < turns) fetch(blockIdx.x / splits, first);
+  int item = 0;
+  for (int block = blockIdx.x / splits; block < blocks; block += step) {
     float total[kBlocks][kTiles][4] = {};
-    for (int turn = first; turn < turns; turn += stride) {
-      uint32_t u[kBlocks][2][kRuns][kWordsRun];
+    int offset[kBlocks][2];  // !kAligned: of the rows' first bytes in their chunks
+    if constexpr (!kAligned) {
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int r = 0; r < kRuns; ++r)
-#pragma unroll
-            for (int i = 0; i < kWordsRun; ++i) u[b][h][r][i] = w[b][h][r][i];
+          offset[b][h] = static_cast<int>(reinterpret_cast<uintptr_t>(a.codes + min(block * kRows + 16 * b + 8 * h + g, a.N - 1) * a.ldw) & 15);
+    }
+    for (int turn = first; turn < turns; turn += stride, ++item) {
+      __syncwarp();  // every lane is done with the stage that the next copy fills, and with the scales
+      copy();
+      keep();
       if (turn + stride < turns) fetch(block, turn + stride);
-      else fetch(block + step, first);
-#pragma unroll
-      for (int r = 0; r < kRuns; ++r) {
-        const int k0 = turn * kTileK + r * 4 * kRun, k = k0 + t * kRun;
-        if (k0 >= K) break;
-        const int group = k0 / a.group;
-        float part[kBlocks][kTiles][4] = {};
-        uint32_t zero[kBlocks][2], zero16[kBlocks][2];
-        float scale[kBlocks][2];
+      else if (block + step < blocks) fetch(block + step, first);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      __syncwarp();
+      const uint32_t* const words = reinterpret_cast<const uint32_t*>(&mine.codes[item % kStages][0][0]);
+      const int k0 = turn * kTileK, runs = min(kTurnRuns, (K - k0 + 31) / 32), g0 = k0 / a.group;
+      int group = 0, end = (g0 + 1) * a.group - k0;  // of the current group, in columns of the turn
+      float part[kBlocks][kTiles][4] = {};
+      uint32_t zero[kBlocks][2];
+      const auto zeros = [&] {
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int64_t at = static_cast<int64_t>(min(block * kRows + 16 * b + 8 * h + g, a.N - 1)) * a.parts + group;
-            scale[b][h] = scale_value(a.scales, a.scale_type, at);
-            const uint32_t z = a.zeros ? a.zeros[at] & 255u : 8u;
-            if constexpr (X::kBf16) {
-              // 128 + z, rounded where z is above 127 (a zero point is meant to be 0..15)
-              const uint32_t v = __bfloat16_as_ushort(__float2bfloat16_rn(128.0f + static_cast<float>(z)));
-              zero[b][h] = v | v << 16;
-              zero16[b][h] = 0;
-            } else {
-              const uint32_t v = __half_as_ushort(__float2half_rn(1024.0f + static_cast<float>(z)));
-              const uint32_t v16 = __half_as_ushort(__float2half_rn(-64.0f - static_cast<float>(z)));
-              zero[b][h] = v | v << 16;
-              zero16[b][h] = v16 | v16 << 16;
-            }
-          }
+          for (int h = 0; h < 2; ++h) zero[b][h] = mine.zero[group][16 * b + 8 * h + g];
+      };
+      zeros();
+#pragma unroll 2
+      for (int r = 0; r < runs; ++r) {
+        uint32_t xb[kTiles][X::kParts][4];
 #pragma unroll
-        for (int i = 0; i < kWordsRun; ++i) {
-          uint32_t xb[kTiles][X::kParts][4];
-#pragma unroll
-          for (int c = 0; c < kTiles; ++c) {
-            uint32_t xw[X::kWords];
-            const int left = 8 * c + g < live ? K - (k + 8 * i) : 0;
-            load_x<kType, kVec>(xrow[c], k + 8 * i, left, xw);
-            split_x<kType>(xw, xb[c]);
-          }
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) {
-            uint32_t p0[4], p1[4];
-            split_codes<X::kBf16>(u[b][0][r][i], zero[b][0], zero16[b][0], p0);
-            split_codes<X::kBf16>(u[b][1][r][i], zero[b][1], zero16[b][1], p1);
-#pragma unroll
-            for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-              for (int q = 0; q < X::kParts; ++q) {
-                mma<X::kBf16>(part[b][c], p0[0], p1[0], p0[1], p1[1], xb[c][q][0], xb[c][q][1]);
-                mma<X::kBf16>(part[b][c], p0[2], p1[2], p0[3], p1[3], xb[c][q][2], xb[c][q][3]);
-              }
-          }
+        for (int c = 0; c < kTiles; ++c) {
+          uint32_t xw[X::kWords];
+          const int m = 8 * c + g, k = k0 + 32 * r + 8 * t;
+          load_x<kType>(x + m * a.ldx * X::kBytes, k, m < live ? K - k : 0, xvec, xw);
+          split_x<kType>(xw, xb[c]);
         }
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+          uint32_t p[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = 16 * b + 8 * h + g;
+            uint32_t u;
+            if constexpr (kAligned) {
+              u = words[row * kChunks * 4 + ((r ^ (row & 7)) * 4 + t)];
+            } else {
+              const int at = row * kChunks * 4 + r * 4 + t + (offset[b][h] >> 2);
+              u = __funnelshift_r(words[at], words[min(at + 1, kRows * kChunks * 4 - 1)], 8 * (offset[b][h] & 3));
+            }
+            if constexpr (X::kBf16) split_codes<true>(u, zero[b][h], 0, p[h]);
+            else split_codes<false>(u, zero[b][h], h2_sub(0x63806380u, zero[b][h]), p[h]);  // 960 - (1024 + z)
+          }
+#pragma unroll
+          for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+            for (int q = 0; q < X::kParts; ++q) {
+              mma<X::kBf16>(part[b][c], p[0][0], p[1][0], p[0][1], p[1][1], xb[c][q][0], xb[c][q][1]);
+              mma<X::kBf16>(part[b][c], p[0][2], p[1][2], p[0][3], p[1][3], xb[c][q][2], xb[c][q][3]);
+            }
+        }
+        if (32 * r + 32 < end && r + 1 < runs) continue;
         // the group's sums, scaled: rows g and g + 8, columns (activation rows) 2 t and 2 t + 1
 #pragma unroll
         for (int c = 0; c < kTiles; ++c) {
@@ -307,12 +337,20 @@ __global__ void __launch_bounds__(32 * kWarps, kTiles == 4 ? 1 : 2) int4_kernel(
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const int m = 8 * c + 2 * t + j;
-              xs[j] = m < live ? a.x_scales[static_cast<int64_t>(m0 + m) * a.parts + group] : 0.0f;
+              xs[j] = m < live ? a.x_scales[static_cast<int64_t>(m0 + m) * a.parts + g0 + group] : 0.0f;
             }
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) total[b][c][j] = fmaf(scale[b][j >> 1] * xs[j & 1], part[b][c][j], total[b][c][j]);
+            for (int j = 0; j < 4; ++j) {
+              total[b][c][j] = fmaf(mine.scale[group][16 * b + 8 * (j >> 1) + g] * xs[j & 1], part[b][c][j], total[b][c][j]);
+              part[b][c][j] = 0.0f;
+            }
+        }
+        if (r + 1 < runs) {
+          ++group;
+          end += a.group;
+          zeros();
         }
       }
     }
@@ -321,7 +359,7 @@ __global__ void __launch_bounds__(32 * kWarps, kTiles == 4 ? 1 : 2) int4_kernel(
 #pragma unroll
       for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s_part[buf][warp][8 * c + 2 * t + (j & 1)][16 * b + 8 * (j >> 1) + g] = total[b][c][j];
+        for (int j = 0; j < 4; ++j) sh.part[warp][8 * c + 2 * t + (j & 1)][16 * b + 8 * (j >> 1) + g] = total[b][c][j];
     __syncthreads();
     // the warps' sums, always in the same order; in a cluster, into the first warp's place for the other CTAs
     const auto put = [&](int m, float v) {
@@ -333,16 +371,19 @@ __global__ void __launch_bounds__(32 * kWarps, kTiles == 4 ? 1 : 2) int4_kernel(
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
       const int m = warp + kWarps * i;
+      if (m >= live) break;
       float v = 0.0f;
 #pragma unroll
-      for (int q = 0; q < kWarps; ++q) v += s_part[buf][q][m][lane];
+      for (int q = 0; q < kWarps; ++q) v += sh.part[q][m][lane];
       if (splits == 1) put(m, v);
-      else s_part[buf][0][m][lane] = v;  // read by this warp alone before
+      else sh.part[0][m][lane] = v;  // row m is read by this warp alone before
     }
-    if (splits > 1) {
+    if (splits == 1) {
+      __syncthreads();
+    } else {
       cluster_sync();
-      for (int m = rank * kWarps + warp; m < kCols; m += splits * kWarps) {
-        const uint32_t at = smem_u32(&s_part[buf][0][m][lane]);
+      for (int m = rank * kWarps + warp; m < live; m += splits * kWarps) {
+        const uint32_t at = smem_u32(&sh.part[0][m][lane]);
         float v = 0.0f;
         for (int q = 0; q < splits; ++q) {
           float o;
@@ -351,25 +392,30 @@ __global__ void __launch_bounds__(32 * kWarps, kTiles == 4 ? 1 : 2) int4_kernel(
         }
         put(m, v);
       }
-      cluster_sync();  // before a peer's buffer is written again, or its CTA ends
-    } else if (kBuffers == 1) {
-      __syncthreads();
+      cluster_sync();  // before a peer's sums are written again, or its CTA ends
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <int kType, int kTiles, int kRun, bool kVec>
-cudaError_t int4_launch(const Int4Args& a, int sms, int m0, cudaStream_t s) {
+template <int kType, int kTiles, bool kAligned>
+cudaError_t int4_launch(const Int4Args& a, int sms, int m0, bool xvec, cudaStream_t s) {
   const int blocks = static_cast<int>(ceil_div(a.N, 32)), turns = static_cast<int>(ceil_div(a.K, kTileK));
   // Columns split over a cluster's CTAs as long as that leaves every warp a turn and the CTAs fit the SMs; by the
   // weights' shape alone, so that a row's sums do not depend on how many rows there are.
   int splits = 1;
   while (splits < 8 && blocks * splits * 2 <= 2 * sms && turns > kWarps * splits) splits *= 2;
-  const int wide = 2 * sms / splits;
-  const int ctas = (blocks < wide ? blocks : wide) * splits;
+  using S = Int4Shape<kTiles, kAligned>;
+  const int wide = S::kCtas * sms / splits;
+  constexpr size_t kSmem = sizeof(typename S::Shared);
+  static_assert(S::kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory of the SM");
+  const auto kernel = int4_kernel<kType, kTiles, kAligned>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.gridDim = dim3(static_cast<unsigned>((blocks < wide ? blocks : wide) * splits));
   cfg.blockDim = dim3(32 * kWarps);
+  cfg.dynamicSmemBytes = kSmem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -377,16 +423,16 @@ cudaError_t int4_launch(const Int4Args& a, int sms, int m0, cudaStream_t s) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = splits > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, int4_kernel<kType, kTiles, kRun, kVec>, a, splits, m0);
+  return cudaLaunchKernelEx(&cfg, kernel, a, splits, m0, xvec);
 }
 
-template <int kType, int kRun, bool kVec>
-cudaError_t int4_rows(const Int4Args& a, int sms, cudaStream_t s) {
+template <int kType, bool kAligned>
+cudaError_t int4_rows(const Int4Args& a, int sms, bool xvec, cudaStream_t s) {
   for (int m0 = 0; m0 < a.M; m0 += 32) {
     const int left = a.M - m0;
-    const cudaError_t e = left <= 8    ? int4_launch<kType, 1, kRun, kVec>(a, sms, m0, s)
-                          : left <= 16 ? int4_launch<kType, 2, kRun, kVec>(a, sms, m0, s)
-                                       : int4_launch<kType, 4, kRun, kVec>(a, sms, m0, s);
+    const cudaError_t e = left <= 8    ? int4_launch<kType, 1, kAligned>(a, sms, m0, xvec, s)
+                          : left <= 16 ? int4_launch<kType, 2, kAligned>(a, sms, m0, xvec, s)
+                                       : int4_launch<kType, 4, kAligned>(a, sms, m0, xvec, s);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -394,13 +440,9 @@ cudaError_t int4_rows(const Int4Args& a, int sms, cudaStream_t s) {
 
 template <int kType>
 cudaError_t int4_type(const Int4Args& a, int sms, cudaStream_t s) {
-  const int run = a.group % 128 == 0 ? 32 : a.group % 64 == 0 ? 16 : 8;
   const int xb = RowType<kType>::kBytes, chunk = xb == 1 ? 8 : 16;  // bytes of an access to x
-  const bool vec = reinterpret_cast<uintptr_t>(a.codes) % (run / 2) == 0 && (a.ldw % (run / 2) == 0 || a.N == 1) &&
-                   reinterpret_cast<uintptr_t>(a.x) % chunk == 0 && (a.ldx * xb % chunk == 0 || a.M == 1);
-  if (run == 32) return vec ? int4_rows<kType, 32, true>(a, sms, s) : int4_rows<kType, 32, false>(a, sms, s);
-  if (run == 16) return vec ? int4_rows<kType, 16, true>(a, sms, s) : int4_rows<kType, 16, false>(a, sms, s);
-  return vec ? int4_rows<kType, 8, true>(a, sms, s) : int4_rows<kType, 8, false>(a, sms, s);
+  const bool xvec = reinterpret_cast<uintptr_t>(a.x) % chunk == 0 && (a.ldx * xb % chunk == 0 || a.M == 1);
+  return aligned16(a.codes) && (a.ldw % 16 == 0 || a.N == 1) ? int4_rows<kType, true>(a, sms, xvec, s) : int4_rows<kType, false>(a, sms, xvec, s);
 }
 
 }  // namespace
