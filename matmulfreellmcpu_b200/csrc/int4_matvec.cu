@@ -33,14 +33,6 @@ constexpr int kTileK = 256;     // columns of a warp's turn (128 bytes of a weig
 constexpr int kTurnRuns = kTileK / 32;  // runs: 32 columns, 8 of each of the 4 lanes that share a row
 constexpr int kPitch = 36;      // words of a partial-sum row of 32 outputs: keeps its writers on different banks
 
-__device__ __forceinline__ float scale_value(const void* p, int type, int64_t i) {
-  switch (type) {
-    case MMFREE_T_F32: return static_cast<const float*>(p)[i];
-    case MMFREE_T_BF16: return to_f32(static_cast<const __nv_bfloat16*>(p)[i]);
-    default: return to_f32(static_cast<const __half*>(p)[i]);
-  }
-}
-
 __device__ __forceinline__ void put_out(void* p, int type, int64_t i, float v) {
   switch (type) {
     case MMFREE_T_F32: static_cast<float*>(p)[i] = v; break;
@@ -74,32 +66,33 @@ struct RowType {
   static constexpr int kWords = 2 * kBytes;  // of 8 elements
 };
 
-// Eight elements of a row from column k, `left` of them inside it (the others are 0).
+// Eight elements of a row from an aligned address.
 template <int kType>
-__device__ __forceinline__ void load_x(const char* row, int k, int left, bool vec, uint32_t (&w)[RowType<kType>::kWords]) {
-  constexpr int kBytes = RowType<kType>::kBytes, kWords = RowType<kType>::kWords;
-  if (vec && left >= 8) {
-    const char* p = row + static_cast<int64_t>(k) * kBytes;
-    if constexpr (kWords == 2) {
-      const uint2 v = *reinterpret_cast<const uint2*>(p);
-      w[0] = v.x, w[1] = v.y;
-    } else {
+__device__ __forceinline__ void load_x(const char* p, uint32_t (&w)[RowType<kType>::kWords]) {
+  if constexpr (RowType<kType>::kWords == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
 #pragma unroll
-      for (int i = 0; i < kWords; i += 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p + 4 * i);
-        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
-      }
+    for (int i = 0; i < RowType<kType>::kWords; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + 4 * i);
+      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
     }
-    return;
   }
+}
+
+// The same from any address, `left` of them inside the row (the others are 0).
+template <int kType>
+__device__ __forceinline__ void load_x_part(const char* p, int left, uint32_t (&w)[RowType<kType>::kWords]) {
+  constexpr int kBytes = RowType<kType>::kBytes;
 #pragma unroll
-  for (int i = 0; i < kWords; ++i) w[i] = 0;
+  for (int i = 0; i < RowType<kType>::kWords; ++i) w[i] = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     if (i >= left) break;
-    if constexpr (kBytes == 4) w[i] = reinterpret_cast<const uint32_t*>(row)[k + i];
-    else if constexpr (kBytes == 2) w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[k + i]) << (16 * (i & 1));
-    else w[i / 4] |= static_cast<uint32_t>(reinterpret_cast<const uint8_t*>(row)[k + i]) << (8 * (i & 3));
+    if constexpr (kBytes == 4) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    else if constexpr (kBytes == 2) w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i]) << (16 * (i & 1));
+    else w[i / 4] |= static_cast<uint32_t>(reinterpret_cast<const uint8_t*>(p)[i]) << (8 * (i & 3));
   }
 }
 
@@ -196,7 +189,7 @@ struct Int4Shape {
 // touches are copied (a chunk with a byte of the row in it can be read as a whole) and its words put together from
 // two, shifted by the row's own offset.
 template <int kType, int kTiles, bool kAligned>
-__global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCtas) int4_kernel(Int4Args a, int splits, int m0, bool xvec) {
+__global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCtas) int4_kernel(Int4Args a, int splits, int m0, bool xvec, uint32_t group_inverse) {
   using X = RowType<kType>;
   using S = Int4Shape<kTiles, kAligned>;
   constexpr int kBlocks = S::kBlocks, kRows = S::kRows, kCols = S::kCols, kChunks = S::kChunks, kStages = S::kStages;
@@ -210,23 +203,34 @@ __global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCta
   const int live = min(kCols, a.M - m0);
   const char* const x = static_cast<const char*>(a.x) + static_cast<int64_t>(m0) * a.ldx * X::kBytes;
 
+  // k / group: columns are below 2^16, where the high word of the product with ceil(2^32 / group) is exact
+  const auto group_of = [&](int k) { return static_cast<int>(__umulhi(static_cast<uint32_t>(k), group_inverse)); };
+
   // the next turn to copy
   int copy_block = blockIdx.x / splits, copy_turn = first, copied = 0;
   const auto copy = [&] {
     if (copy_block < blocks && first < turns) {
       const uint32_t to = smem_u32(&mine.codes[copied % kStages][0][0]);
-      const int from = copy_turn * (kTileK / 2);
-      for (int i = lane; i < kRows * kChunks; i += 32) {
-        const int row = i / kChunks, c = i % kChunks;
-        const uint8_t* const line = a.codes + min(copy_block * kRows + row, a.N - 1) * a.ldw;
-        if constexpr (kAligned) {
-          const int at = from + 16 * c, left = min(max(bytes - at, 0), 16);
-          // chunks of a row are rotated by the row, so that 8 rows' words of one column are on different banks
-          copy16(to + (row * kChunks + (c ^ (row & 7))) * 16, left ? line + at : line, left);
-        } else {
-          const uint8_t* const at = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(line + from) & ~uintptr_t(15)) + 16 * c;
-          const bool any = at < line + bytes;
-          copy16(to + i * 16, any ? at : reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(line) & ~uintptr_t(15)), any ? 16 : 0);
+      const int from = copy_turn * (kTileK / 2), n0 = copy_block * kRows;
+      if constexpr (kAligned) {
+        // lane: chunk lane % 8 of every fourth row; chunks of a row are exchanged by the row, so that 8 rows' words of
+        // one column are on different banks
+        const int c = lane & 7, at = from + 16 * c, left = min(max(bytes - at, 0), 16);
+        const uint8_t* line = a.codes + (n0 + (lane >> 3)) * a.ldw + (left ? at : 0);
+        const int64_t rows4 = 4 * a.ldw;
+#pragma unroll
+        for (int i = 0; i < kRows / 4; ++i, line += rows4) {
+          const int row = (lane >> 3) + 4 * i;
+          if (n0 + row >= a.N) break;  // rows behind the last: what the stage held
+          copy16(to + (row * 8 + (c ^ (row & 7))) * 16, line, left);
+        }
+      } else {
+        for (int i = lane; i < kRows * kChunks; i += 32) {
+          const int row = i / kChunks, c = i % kChunks;
+          const uint8_t* const line = a.codes + min(n0 + row, a.N - 1) * a.ldw;
+          const uintptr_t at = (reinterpret_cast<uintptr_t>(line + from) & ~uintptr_t(15)) + 16 * c;
+          const bool any = at < reinterpret_cast<uintptr_t>(line + bytes);
+          copy16(to + i * 16, reinterpret_cast<const void*>(any ? at : reinterpret_cast<uintptr_t>(line) & ~uintptr_t(15)), any ? 16 : 0);
         }
       }
       if ((copy_turn += stride) >= turns) copy_turn = first, copy_block += step;
@@ -234,32 +238,34 @@ __global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCta
     ++copied;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // scales and zero points of a turn: lane r has row r's, up to 8 groups
-  float next_scale[kTurnRuns];
-  uint32_t next_zero[kTurnRuns];
+  // scales and zero points of a turn: lane r has row r's, of up to 8 groups, as they lie in memory
+  uint32_t next_scale[kTurnRuns], next_zero[kTurnRuns];
+  int next_groups = 0;
+  const bool wide_scales = a.scale_type == MMFREE_T_F32;
   const auto fetch = [&](int block, int turn) {
-    const int64_t at = static_cast<int64_t>(min(block * kRows + lane, a.N - 1)) * a.parts;
-    const int g0 = turn * kTileK / a.group, g1 = min(a.parts - 1, (turn * kTileK + kTileK - 1) / a.group);
+    const int g0 = group_of(turn * kTileK), g1 = min(a.parts - 1, group_of(turn * kTileK + kTileK - 1));
+    const int64_t at = static_cast<int64_t>(min(block * kRows + lane, a.N - 1)) * a.parts + g0;
+    const char* const p = static_cast<const char*>(a.scales) + at * (wide_scales ? 4 : 2);
+    next_groups = g1 - g0 + 1;
 #pragma unroll
     for (int i = 0; i < kTurnRuns; ++i) {
-      if (g0 + i > g1) break;
-      next_scale[i] = scale_value(a.scales, a.scale_type, at + g0 + i);
-      next_zero[i] = a.zeros ? a.zeros[at + g0 + i] : 8u;
+      if (i >= next_groups) break;
+      next_scale[i] = wide_scales ? reinterpret_cast<const uint32_t*>(p)[i] : reinterpret_cast<const uint16_t*>(p)[i];
+      next_zero[i] = a.zeros ? a.zeros[at + i] : 8u;
     }
   };
   const auto keep = [&] {
 #pragma unroll
     for (int i = 0; i < kTurnRuns; ++i) {
-      mine.scale[i][lane] = next_scale[i];
-      // 128 + z or 1024 + z twice (z up to 127 is exact)
-      uint32_t v;
-      if constexpr (X::kBf16) v = __bfloat16_as_ushort(__float2bfloat16_rn(128.0f + static_cast<float>(next_zero[i])));
-      else v = __half_as_ushort(__float2half_rn(1024.0f + static_cast<float>(next_zero[i])));
-      mine.zero[i][lane] = v | v << 16;
+      if (i >= next_groups) break;
+      mine.scale[i][lane] = a.scale_type == MMFREE_T_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(next_scale[i])))
+                                                         : __uint_as_float(next_scale[i] << (wide_scales ? 0 : 16));
+      // 128 + z or 1024 + z twice (z up to 127 is exact): 0x4300 + z is 128 + z in bf16, 0x6400 + z is 1024 + z in fp16
+      mine.zero[i][lane] = (X::kBf16 ? 0x43004300u : 0x64006400u) + next_zero[i] * 0x10001u;
     }
   };
 #pragma unroll
-  for (int i = 0; i < kTurnRuns; ++i) next_scale[i] = 0.0f, next_zero[i] = 0;
+  for (int i = 0; i < kTurnRuns; ++i) next_scale[i] = next_zero[i] = 0;
 #pragma unroll
   for (int i = 0; i + 1 < kStages; ++i) copy();
   if (blockIdx.x / splits < blocks && first < turns) fetch(blockIdx.x / splits, first);
@@ -283,74 +289,91 @@ __global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCta
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       __syncwarp();
       const uint32_t* const words = reinterpret_cast<const uint32_t*>(&mine.codes[item % kStages][0][0]);
-      const int k0 = turn * kTileK, runs = min(kTurnRuns, (K - k0 + 31) / 32), g0 = k0 / a.group;
-      int group = 0, end = (g0 + 1) * a.group - k0;  // of the current group, in columns of the turn
-      float part[kBlocks][kTiles][4] = {};
-      uint32_t zero[kBlocks][2];
-      const auto zeros = [&] {
+      const int k0 = turn * kTileK, runs = min(kTurnRuns, (K - k0 + 31) / 32), g0 = group_of(k0);
+      // a whole turn of aligned rows is read without a test (lanes of absent rows read the last one: their columns of
+      // the result are not stored)
+      const bool whole = xvec && k0 + kTileK <= K;
+      const char* xp[kTiles];
+#pragma unroll
+      for (int c = 0; c < kTiles; ++c) xp[c] = x + (static_cast<int64_t>(min(8 * c + g, live - 1)) * a.ldx + k0 + 8 * t) * X::kBytes;
+      int r = 0;
+#pragma unroll 1
+      for (int group = 0; r < runs; ++group) {
+        const int stop = min(runs, ((g0 + group + 1) * a.group - k0) / 32);
+        float part[kBlocks][kTiles][4] = {};
+        uint32_t zero[kBlocks][2], zero16[kBlocks][2];
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) zero[b][h] = mine.zero[group][16 * b + 8 * h + g];
-      };
-      zeros();
-#pragma unroll 2
-      for (int r = 0; r < runs; ++r) {
-        uint32_t xb[kTiles][X::kParts][4];
-#pragma unroll
-        for (int c = 0; c < kTiles; ++c) {
-          uint32_t xw[X::kWords];
-          const int m = 8 * c + g, k = k0 + 32 * r + 8 * t;
-          load_x<kType>(x + m * a.ldx * X::kBytes, k, m < live ? K - k : 0, xvec, xw);
-          split_x<kType>(xw, xb[c]);
-        }
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-          uint32_t p[2][4];
-#pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int row = 16 * b + 8 * h + g;
-            uint32_t u;
-            if constexpr (kAligned) {
-              u = words[row * kChunks * 4 + ((r ^ (row & 7)) * 4 + t)];
-            } else {
-              const int at = row * kChunks * 4 + r * 4 + t + (offset[b][h] >> 2);
-              u = __funnelshift_r(words[at], words[min(at + 1, kRows * kChunks * 4 - 1)], 8 * (offset[b][h] & 3));
-            }
-            if constexpr (X::kBf16) split_codes<true>(u, zero[b][h], 0, p[h]);
-            else split_codes<false>(u, zero[b][h], h2_sub(0x63806380u, zero[b][h]), p[h]);  // 960 - (1024 + z)
+            zero[b][h] = mine.zero[group][16 * b + 8 * h + g];
+            zero16[b][h] = X::kBf16 ? 0 : h2_sub(0x63806380u, zero[b][h]);  // 960 - (1024 + z)
           }
+        const auto run = [&](const uint32_t (&xw)[kTiles][X::kWords]) {
+          uint32_t xb[kTiles][X::kParts][4];
 #pragma unroll
-          for (int c = 0; c < kTiles; ++c)
+          for (int c = 0; c < kTiles; ++c) split_x<kType>(xw[c], xb[c]);
 #pragma unroll
-            for (int q = 0; q < X::kParts; ++q) {
-              mma<X::kBf16>(part[b][c], p[0][0], p[1][0], p[0][1], p[1][1], xb[c][q][0], xb[c][q][1]);
-              mma<X::kBf16>(part[b][c], p[0][2], p[1][2], p[0][3], p[1][3], xb[c][q][2], xb[c][q][3]);
+          for (int b = 0; b < kBlocks; ++b) {
+            uint32_t p[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int row = 16 * b + 8 * h + g;
+              uint32_t u;
+              if constexpr (kAligned) {
+                u = words[row * kChunks * 4 + (((r ^ g) & 7) * 4 + t)];
+              } else {
+                const int at = row * kChunks * 4 + r * 4 + t + (offset[b][h] >> 2);
+                u = __funnelshift_r(words[at], words[min(at + 1, kRows * kChunks * 4 - 1)], 8 * (offset[b][h] & 3));
+              }
+              split_codes<X::kBf16>(u, zero[b][h], zero16[b][h], p[h]);
             }
+#pragma unroll
+            for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+              for (int q = 0; q < X::kParts; ++q) {
+                mma<X::kBf16>(part[b][c], p[0][0], p[1][0], p[0][1], p[1][1], xb[c][q][0], xb[c][q][1]);
+                mma<X::kBf16>(part[b][c], p[0][2], p[1][2], p[0][3], p[1][3], xb[c][q][2], xb[c][q][3]);
+              }
+          }
+        };
+        uint32_t xw[kTiles][X::kWords];
+        if (whole) {
+          // each run's rows are loaded a run ahead
+          uint32_t ahead[kTiles][X::kWords];
+#pragma unroll
+          for (int c = 0; c < kTiles; ++c) load_x<kType>(xp[c] + 32 * X::kBytes * r, ahead[c]);
+#pragma unroll 2
+          for (; r < stop; ++r) {
+            const int next = min(r + 1, kTurnRuns - 1);
+#pragma unroll
+            for (int c = 0; c < kTiles; ++c) {
+#pragma unroll
+              for (int i = 0; i < X::kWords; ++i) xw[c][i] = ahead[c][i];
+              load_x<kType>(xp[c] + 32 * X::kBytes * next, ahead[c]);
+            }
+            run(xw);
+          }
+        } else {
+#pragma unroll 1
+          for (; r < stop; ++r) {
+#pragma unroll
+            for (int c = 0; c < kTiles; ++c) load_x_part<kType>(xp[c] + 32 * X::kBytes * r, K - (k0 + 32 * r + 8 * t), xw[c]);
+            run(xw);
+          }
         }
-        if (32 * r + 32 < end && r + 1 < runs) continue;
         // the group's sums, scaled: rows g and g + 8, columns (activation rows) 2 t and 2 t + 1
 #pragma unroll
         for (int c = 0; c < kTiles; ++c) {
           float xs[2] = {1.0f, 1.0f};
           if (a.x_grouped)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int m = 8 * c + 2 * t + j;
-              xs[j] = m < live ? a.x_scales[static_cast<int64_t>(m0 + m) * a.parts + g0 + group] : 0.0f;
-            }
+            for (int j = 0; j < 2; ++j) xs[j] = a.x_scales[static_cast<int64_t>(m0 + min(8 * c + 2 * t + j, live - 1)) * a.parts + g0 + group];
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              total[b][c][j] = fmaf(mine.scale[group][16 * b + 8 * (j >> 1) + g] * xs[j & 1], part[b][c][j], total[b][c][j]);
-              part[b][c][j] = 0.0f;
-            }
-        }
-        if (r + 1 < runs) {
-          ++group;
-          end += a.group;
-          zeros();
+            for (int j = 0; j < 4; ++j)
+              total[b][c][j] = fmaf(mine.scale[group][16 * b + 8 * (j >> 1) + g], part[b][c][j] * xs[j & 1], total[b][c][j]);
         }
       }
     }
@@ -423,7 +446,9 @@ cudaError_t int4_launch(const Int4Args& a, int sms, int m0, bool xvec, cudaStrea
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = splits > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, a, splits, m0, xvec);
+  // a group of 2^16 columns or more is the only one
+  const uint32_t inverse = a.group < 65536 ? static_cast<uint32_t>(((uint64_t(1) << 32) + a.group - 1) / a.group) : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, a, splits, m0, xvec, inverse);
 }
 
 template <int kType, bool kAligned>
