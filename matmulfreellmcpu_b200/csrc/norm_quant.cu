@@ -31,103 +31,160 @@ __device__ __forceinline__ int code_s8(float t, float inv, float m) {
   return e == e ? static_cast<int>(e) : 0;
 }
 
-template <typename T, typename Code, int kChunks, bool kVec>
-__global__ void __launch_bounds__(1024) norm_quant_kernel(NormQuantArgs a) {
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-  T* res = a.residual ? static_cast<T*>(a.residual) + row * a.ldr : nullptr;
-  Code* codes = static_cast<Code*>(a.codes) + row * a.cols;
-  const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5;
-  float t[kChunks][kCols];
-  float sum = 0.0f;
-  uint32_t most[kChunks];  // |t| as its bits: ordered like the values, a NaN above all
-#pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    const int col = (tid + c * static_cast<int>(blockDim.x)) * kCols;
-    const int n = a.cols - col;
-    most[c] = 0;
-    if (n <= 0) continue;
-    load_row<kVec>(x + col, n, t[c]);
-    if (res) {
-      float r[kCols];
-      load_row<kVec>(res + col, n, r);
-#pragma unroll
-      for (int i = 0; i < kCols; ++i) t[c][i] = to_f32(from_f32<T>(r[i] + t[c][i]));
-      store_row<kVec>(res + col, n, t[c]);
-    }
-    float w[kCols];
-    load_row<kVec>(a.weight + col, n, w);
-#pragma unroll
-    for (int i = 0; i < kCols; ++i) {
-      sum = fmaf(t[c][i], t[c][i], sum);
-      t[c][i] = __fmul_rn(t[c][i], w[i]);
-      most[c] = max(most[c], __float_as_uint(t[c][i]) & 0x7FFFFFFFu);
-    }
-  }
-  uint32_t row_most = 0;
-  if (a.group == 0) {
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) row_most = max(row_most, most[c]);
-    row_most = __reduce_max_sync(0xFFFFFFFFu, row_most);
+// Eight columns as they lie in memory, whole or one by one.
+template <typename T, bool kVec>
+__device__ __forceinline__ void fetch8(const T* p, int n, Words<T, kCols>& w) {
+  if constexpr (kVec) {
+    w.load(p);
   } else {
-    // a group is 4, 8 or 16 neighbouring lanes' chunks
+    Pack<T, kCols> k;
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) k.v[i] = i < n ? p[i] : from_f32<T>(0.0f);
+    memcpy(&w.w, &k, sizeof(k));
+  }
+}
+
+// A CTA holds a row in registers, kChunks chunks of 8 columns a thread, and walks the rows with a fixed stride; up to
+// two chunks it also keeps the weights, and loads the next row while this one is reduced and stored.
+template <typename T, typename Code, int kChunks, bool kVec>
+__global__ void __launch_bounds__(kChunks == 1 ? 256 : kChunks == 2 ? 512 : 1024, 1) norm_quant_kernel(NormQuantArgs a) {
+  constexpr bool kAhead = kChunks <= 2;
+  constexpr bool kS8 = std::is_same<Code, int8_t>::value;
+  constexpr float kLimit = kS8 ? 127.0f : 448.0f;
+  __shared__ float s_sum[2][32];
+  __shared__ uint32_t s_most[2][32];
+  const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5;
+  const bool add = a.residual != nullptr;
+  Words<T, kCols> next_x[kChunks], next_r[kChunks];
+  const auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      most[c] = max(most[c], __shfl_xor_sync(0xFFFFFFFFu, most[c], 1));
-      most[c] = max(most[c], __shfl_xor_sync(0xFFFFFFFFu, most[c], 2));
-      if (a.group >= 64) most[c] = max(most[c], __shfl_xor_sync(0xFFFFFFFFu, most[c], 4));
-      if (a.group >= 128) most[c] = max(most[c], __shfl_xor_sync(0xFFFFFFFFu, most[c], 8));
+      const int col = (tid + c * static_cast<int>(blockDim.x)) * kCols, n = a.cols - col;
+      if (n <= 0) break;
+      fetch8<T, kVec>(static_cast<const T*>(a.x) + row * a.ldx + col, n, next_x[c]);
+      if (add) fetch8<T, kVec>(static_cast<const T*>(a.residual) + row * a.ldr + col, n, next_r[c]);
     }
-  }
+  };
+  float w[kAhead ? kChunks : 1][kCols];
+  if constexpr (kAhead) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  if (warps > 1) {
-    __shared__ float s_sum[32];
-    __shared__ uint32_t s_most[32];
-    if (lane == 0) {
-      s_sum[tid >> 5] = sum;
-      s_most[tid >> 5] = row_most;
+    for (int c = 0; c < kChunks; ++c) {
+      const int col = (tid + c * static_cast<int>(blockDim.x)) * kCols;
+      if (col < a.cols) load_row<kVec>(a.weight + col, a.cols - col, w[c]);
     }
-    __syncthreads();
-    // every warp sums all partials in the same order
-    sum = lane < warps ? s_sum[lane] : 0.0f;
-    row_most = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? s_most[lane] : 0u);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    fetch(blockIdx.x);
   }
-  const float rstd = 1.0f / sqrtf(sum / static_cast<float>(a.cols) + a.eps);
-  constexpr bool kS8 = sizeof(Code) == 1 && std::is_same<Code, int8_t>::value;
-  constexpr float kLimit = kS8 ? 127.0f : 448.0f;
-  float* scales = a.scales + row * a.parts;
-  if (a.group == 0 && tid == 0) scales[0] = __uint_as_float(row_most) * rstd / kLimit;
+  int buf = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, buf ^= 1) {
+    if constexpr (!kAhead) fetch(row);
+    float t[kChunks][kCols], sum = 0.0f;
+    uint32_t most[kChunks];  // |t| as its bits: ordered like the values, a NaN above all
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    const int col = (tid + c * static_cast<int>(blockDim.x)) * kCols;
-    const int n = a.cols - col;
-    if (n <= 0) continue;
-    const float m = __uint_as_float(a.group ? most[c] : row_most);
-    if (a.group && (col % a.group) == 0) scales[col / a.group] = m * rstd / kLimit;
-    const float inv = kLimit / m;
-    Pack<uint8_t, kCols> q;
+    for (int c = 0; c < kChunks; ++c) {
+      const int col = (tid + c * static_cast<int>(blockDim.x)) * kCols, n = a.cols - col;
+      most[c] = 0;
+      if (n <= 0) continue;
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) {
-      if constexpr (kS8) {
-        q.v[i] = static_cast<uint8_t>(code_s8(t[c][i], inv, m));
-      } else {
-        float v = t[c][i] * inv;
-        if (!(inv < __int_as_float(0x7F800000)))  // m is 0, too small for its reciprocal, or a NaN
-          v = m == 0.0f ? 0.0f : static_cast<float>(static_cast<double>(t[c][i]) * 448.0 / static_cast<double>(m));
-        q.v[i] = __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+      for (int i = 0; i < kCols; ++i) t[c][i] = next_x[c][i];
+      if (add) {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) t[c][i] = to_f32(from_f32<T>(next_r[c][i] + t[c][i]));
+        store_row<kVec>(static_cast<T*>(a.residual) + row * a.ldr + col, n, t[c]);
+      }
+      if constexpr (!kAhead) load_row<kVec>(a.weight + col, n, w[0]);
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) {
+        sum = fmaf(t[c][i], t[c][i], sum);
+        t[c][i] = __fmul_rn(t[c][i], w[kAhead ? c : 0][i]);
+        most[c] = max(most[c], __float_as_uint(t[c][i]) & 0x7FFFFFFFu);
       }
     }
-    if constexpr (kVec) {
-      *reinterpret_cast<Pack<uint8_t, kCols>*>(codes + col) = q;
-    } else {
+    if (kAhead && row + gridDim.x < a.rows) fetch(row + gridDim.x);
+    uint32_t row_most = 0;
+    if (a.group == 0) {
 #pragma unroll
-      for (int i = 0; i < kCols; ++i)
-        if (i < n) reinterpret_cast<uint8_t*>(codes)[col + i] = q.v[i];
+      for (int c = 0; c < kChunks; ++c) row_most = max(row_most, most[c]);
+      row_most = __reduce_max_sync(0xFFFFFFFFu, row_most);
+    } else {
+      // a group is 4, 8 or 16 neighbouring lanes' chunks
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        most[c] = max(most[c], __shfl_xor_sync(0xFFFFFFFFu, most[c], 1));
+        most[c] = max(most[c], __shfl_xor_sync(0xFFFFFFFFu, most[c], 2));
+        if (a.group >= 64) most[c] = max(most[c], __shfl_xor_sync(0xFFFFFFFFu, most[c], 4));
+        if (a.group >= 128) most[c] = max(most[c], __shfl_xor_sync(0xFFFFFFFFu, most[c], 8));
+      }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (warps > 1) {
+      if (lane == 0) {
+        s_sum[buf][tid >> 5] = sum;
+        s_most[buf][tid >> 5] = row_most;
+      }
+      __syncthreads();  // one a row: the next row's partials go to the other half
+      // every warp sums all partials in the same order
+      sum = lane < warps ? s_sum[buf][lane] : 0.0f;
+      row_most = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? s_most[buf][lane] : 0u);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    }
+    const float rstd = 1.0f / sqrtf(sum / static_cast<float>(a.cols) + a.eps);
+    float* const scales = a.scales + row * a.parts;
+    if (a.group == 0 && tid == 0) scales[0] = __uint_as_float(row_most) * rstd / kLimit;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const int col = (tid + c * static_cast<int>(blockDim.x)) * kCols, n = a.cols - col;
+      if (n <= 0) continue;
+      const float m = __uint_as_float(a.group ? most[c] : row_most);
+      if (a.group && (col & (a.group - 1)) == 0) scales[col / a.group] = m * rstd / kLimit;
+      const float inv = kLimit / m;
+      Pack<uint8_t, kCols> q;
+      if constexpr (kS8) {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) q.v[i] = static_cast<uint8_t>(code_s8(t[c][i], inv, m));
+      } else {
+        if (inv < __int_as_float(0x7F800000)) {
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) t[c][i] *= inv;
+        } else {  // m is 0, too small for its reciprocal, or a NaN
+#pragma unroll
+          for (int i = 0; i < kCols; ++i)
+            t[c][i] = m == 0.0f ? 0.0f : static_cast<float>(static_cast<double>(t[c][i]) * 448.0 / static_cast<double>(m));
+        }
+#pragma unroll
+        for (int i = 0; i < kCols; i += 2) {
+          const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(make_float2(t[c][i], t[c][i + 1]), __NV_SATFINITE, __NV_E4M3);
+          q.v[i] = static_cast<uint8_t>(two);
+          q.v[i + 1] = static_cast<uint8_t>(two >> 8);
+        }
+      }
+      uint8_t* const codes = static_cast<uint8_t*>(a.codes) + row * a.cols + col;
+      if constexpr (kVec) {
+        *reinterpret_cast<Pack<uint8_t, kCols>*>(codes) = q;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i)
+          if (i < n) codes[i] = q.v[i];
+      }
     }
   }
+}
+
+template <typename T, typename Code, int kChunks, bool kVec>
+cudaError_t launch_chunks(const NormQuantArgs& a, int threads, cudaStream_t s) {
+  // as many CTAs as the SMs hold at once, each with its share of the rows
+  const auto kernel = norm_quant_kernel<T, Code, kChunks, kVec>;
+  int64_t grid = a.rows;
+  if (grid > 148) {
+    int dev = 0, sms = 0, held = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, threads, 0);
+    if (e != cudaSuccess) return e;
+    if (grid > static_cast<int64_t>(sms) * held) grid = static_cast<int64_t>(sms) * held;
+  }
+  return launch_k(kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), 0, s, false, a);
 }
 
 template <typename T, typename Code, bool kVec>
@@ -136,12 +193,11 @@ cudaError_t launch_cols(const NormQuantArgs& a, cudaStream_t s) {
   // a thread holds 1 to 8 chunks of the row in registers
   const int per = chunks <= 256 ? 1 : chunks <= 1024 ? 2 : chunks <= 4096 ? 4 : 8;
   const int threads = static_cast<int>(ceil_div(ceil_div(chunks, per), 32) * 32);
-  const dim3 grid(static_cast<unsigned>(a.rows));
   switch (per) {
-    case 1: return launch_k(norm_quant_kernel<T, Code, 1, kVec>, grid, dim3(threads), 0, s, false, a);
-    case 2: return launch_k(norm_quant_kernel<T, Code, 2, kVec>, grid, dim3(threads), 0, s, false, a);
-    case 4: return launch_k(norm_quant_kernel<T, Code, 4, kVec>, grid, dim3(threads), 0, s, false, a);
-    default: return launch_k(norm_quant_kernel<T, Code, 8, kVec>, grid, dim3(threads), 0, s, false, a);
+    case 1: return launch_chunks<T, Code, 1, kVec>(a, threads, s);
+    case 2: return launch_chunks<T, Code, 2, kVec>(a, threads, s);
+    case 4: return launch_chunks<T, Code, 4, kVec>(a, threads, s);
+    default: return launch_chunks<T, Code, 8, kVec>(a, threads, s);
   }
 }
 

@@ -49,12 +49,16 @@ __device__ __forceinline__ int64_t sequence_slot(const int32_t* slots, int64_t c
 
 template <int W, int V>
 __device__ __forceinline__ void conv_load_taps(const mmfree_cuda_conv_args& a, int64_t d, float (&w)[V][W], float (&bias)[V]) {
+  if constexpr (V > 1) {  // 16-byte loads: the channels' taps lie one behind another
+    const Pack<float, V * W> p = *reinterpret_cast<const Pack<float, V * W>*>(a.weight + d * W);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+    for (int i = 0; i < V * W; ++i) w[i / W][i % W] = p.v[i];
+  } else {
 #pragma unroll
-    for (int j = 0; j < W; ++j) w[i][j] = a.weight[(d + i) * W + j];
-    bias[i] = a.bias ? a.bias[d + i] : 0.0f;
+    for (int j = 0; j < W; ++j) w[0][j] = a.weight[d * W + j];
   }
+#pragma unroll
+  for (int i = 0; i < V; ++i) bias[i] = a.bias ? a.bias[d + i] : 0.0f;
 }
 
 // in: the window's W - 1 older inputs, then the newest; returns the output of each channel.
@@ -157,12 +161,22 @@ __global__ void __launch_bounds__(128) conv_kernel(mmfree_cuda_conv_args a, int 
 #pragma unroll
       for (int j = 0; j < W - 1; ++j) load_row<kVec>(x + (t - (W - 1) + j) * ldx, V, win[j]);
     }
-    for (; t < stop; ++t) {
-      float v[V], y[V];
-      load_row<kVec>(x + t * ldx, V, v);
-      conv_token<W, V>(win, v, w, bias, silu, y);
-      store_row<kVec>(out + t * ldo, V, y);
-      conv_shift<W, V>(win, v);
+    // eight tokens' loads in flight together (those behind the last read it again)
+    constexpr int kBatch = 8;
+    for (; t < stop; t += kBatch) {
+      Words<T, V> raw[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) raw[k].load(x + min(t + k, stop - 1) * ldx);
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (t + k >= stop) break;
+        float v[V], y[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = raw[k][i];
+        conv_token<W, V>(win, v, w, bias, silu, y);
+        store_row<kVec>(out + (t + k) * ldo, V, y);
+        conv_shift<W, V>(win, v);
+      }
     }
   }
 }
@@ -199,7 +213,9 @@ cudaError_t conv_launch(const mmfree_cuda_conv_args& a, bool step, cudaStream_t 
   const unsigned blocks = static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.channels), 128 * V));
   mark_device();
   if (step) return launch_k(conv_step_kernel<T, W, V>, dim3(blocks, static_cast<unsigned>(a.seqs)), dim3(128), 0, s, false, a);
-  int rows = 32;
+  // tokens of a tile: 64, of which W - 1 are read twice, fewer where the tiles would not fill the SMs (a small call)
+  int rows = 64;
+  while (rows > 8 && static_cast<int64_t>(blocks) * ceil_div(static_cast<int64_t>(a.tokens), rows) < 4 * 148) rows /= 2;
   while (ceil_div(static_cast<int64_t>(a.tokens), rows) > 65535) rows *= 2;  // grid.y is 16 bits
   const unsigned tiles = static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.tokens), rows));
   return launch_k(conv_kernel<T, W, V>, dim3(blocks, tiles), dim3(128), 0, s, false, a, rows);
@@ -223,7 +239,7 @@ template <typename T>
 cudaError_t conv_type(const mmfree_cuda_conv_args& a, bool step, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);  // channels of a 16-byte access
   const bool vec = a.channels % V == 0 && a.ldx % V == 0 && a.ld_out % V == 0 && aligned16(a.x) && aligned16(a.out) &&
-                   aligned16(a.state);
+                   aligned16(a.state) && aligned16(a.weight);
   return vec ? conv_width<T, V>(a, step, s) : conv_width<T, 1>(a, step, s);
 }
 
@@ -237,58 +253,64 @@ cudaError_t conv_any(const mmfree_cuda_conv_args& a, bool step, cudaStream_t s) 
 
 // ---- selective scan --------------------------------------------------------------------------
 
-__device__ __forceinline__ float softplus_f32(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
+// softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) <= 1, with log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1/3,
+// by its series 2 (s + s^3/3 + s^5/5 + ...): the first term left out is below 2^-25 of the sum. Exact to a few
+// steps for all v, where log(1 + e) rounded first would lose small e. Two special-function operations.
+__device__ __forceinline__ float softplus_f32(float v) {
+  const float e = ex2(-fabsf(v) * kLog2E);
+  const float s = e * rcp(2.0f + e), q = s * s;
+  float p = 1.0f / 15.0f;
+  p = fmaf(p, q, 1.0f / 13.0f);
+  p = fmaf(p, q, 1.0f / 11.0f);
+  p = fmaf(p, q, 1.0f / 9.0f);
+  p = fmaf(p, q, 1.0f / 7.0f);
+  p = fmaf(p, q, 1.0f / 5.0f);
+  p = fmaf(p, q, 1.0f / 3.0f);
+  const float l = fmaf(s * q, p, s);
+  return fmaf(2.0f, l, fmaxf(v, 0.0f));
+}
 
-constexpr int kMaxPerLane = MMFREE_CUDA_MAX_STATES / 32;
-
-// `lanes` lanes (a power of two) per (sequence, channel), each holding every lanes-th state.
-template <typename T>
-__global__ void __launch_bounds__(128) ssm_kernel(mmfree_cuda_ssm_args a, int lanes, bool step) {
-  const int64_t channels = static_cast<int64_t>(a.channels), states = static_cast<int64_t>(a.states);
-  const int lane = threadIdx.x & (lanes - 1);
-  const int64_t d = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes;
-  const bool live = d < channels;
-  const int64_t dd = live ? d : channels - 1, seq = blockIdx.y;
-  int64_t b = seq, e = seq + 1;
-  if (!step && !sequence_rows(a.seq_starts, static_cast<int64_t>(a.tokens), seq, b, e)) return;
-  if (b == e) return;
+// One token of a stream: `lanes` lanes (a power of two) a channel, kStates neighbouring states a lane, kVec: read and
+// written by 16 bytes. Bound by the state's bytes; every lane repeats its channel's softplus and gate, which costs less
+// than passing them on.
+template <typename T, int kStates, bool kVec>
+__global__ void __launch_bounds__(256) step_kernel(mmfree_cuda_ssm_args a, int lanes) {
+  const int64_t channels = static_cast<int64_t>(a.channels);
+  const int states = static_cast<int>(a.states), lane = threadIdx.x & (lanes - 1);
+  const int64_t d = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes, seq = blockIdx.y;
   const int64_t slot = sequence_slot(a.slots, static_cast<int64_t>(a.slot_count), seq);
   if (slot < 0) return;
-  float* state = a.state ? a.state + (slot * channels + dd) * states : nullptr;
-  float h[kMaxPerLane], rate[kMaxPerLane];
-#pragma unroll
-  for (int j = 0; j < kMaxPerLane; ++j) {
-    const int64_t n = lane + j * lanes;
-    const bool in = n < states;
-    h[j] = in && state ? state[n] : 0.0f;
-    rate[j] = in ? a.A[dd * states + n] : 0.0f;
-  }
+  const bool live = d < channels;
+  const int64_t dd = live ? d : channels - 1;
+  const int n = lane * kStates, left = states - n;
+  float* const state = a.state + (slot * channels + dd) * states + n;
+  const float* const rates = a.A + dd * states + n;
   const int64_t group = dd / (channels / static_cast<int64_t>(a.groups));
-  const float skip = a.D ? a.D[dd] : 0.0f, bias = a.dt_bias ? a.dt_bias[dd] : 0.0f;
-  for (int64_t t = b; t < e; ++t) {
-    const float x = to_f32(static_cast<const T*>(a.x)[t * static_cast<int64_t>(a.ldx) + dd]);
-    float delta = to_f32(static_cast<const T*>(a.dt)[t * static_cast<int64_t>(a.ld_dt) + dd]) + bias;
-    if (a.dt_softplus) delta = softplus_f32(delta);
-    const T* B = static_cast<const T*>(a.B) + t * static_cast<int64_t>(a.ldb) + group * states;
-    const T* C = static_cast<const T*>(a.C) + t * static_cast<int64_t>(a.ldc) + group * states;
-    float y = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kMaxPerLane; ++j) {
-      const int64_t n = lane + j * lanes;
-      if (n < states) {
-        h[j] = fmaf(expf(delta * rate[j]), h[j], delta * x * to_f32(B[n]));
-        y = fmaf(to_f32(C[n]), h[j], y);
-      }
-    }
-    for (int o = lanes >> 1; o; o >>= 1) y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
-    y = fmaf(skip, x, y);
-    if (a.z) y *= silu_f32(to_f32(static_cast<const T*>(a.z)[t * static_cast<int64_t>(a.ldz) + dd]));
-    if (live && lane == 0) static_cast<T*>(a.out)[t * static_cast<int64_t>(a.ld_out) + dd] = from_f32<T>(y);
+  const T* const B = static_cast<const T*>(a.B) + seq * static_cast<int64_t>(a.ldb) + group * states + n;
+  const T* const C = static_cast<const T*>(a.C) + seq * static_cast<int64_t>(a.ldc) + group * states + n;
+  float h[kStates] = {}, rate[kStates] = {}, b[kStates] = {}, c[kStates] = {};
+  if (left > 0) {
+    load_row<kVec>(state, left, h);
+    load_row<kVec>(rates, left, rate);
+    load_row<kVec>(B, left, b);
+    load_row<kVec>(C, left, c);
   }
-  if (state && live)
+  const float x = to_f32(static_cast<const T*>(a.x)[seq * static_cast<int64_t>(a.ldx) + dd]);
+  float delta = to_f32(static_cast<const T*>(a.dt)[seq * static_cast<int64_t>(a.ld_dt) + dd]);
+  const float z = a.z ? to_f32(static_cast<const T*>(a.z)[seq * static_cast<int64_t>(a.ldz) + dd]) : 0.0f;
+  if (a.dt_bias) delta += a.dt_bias[dd];
+  if (a.dt_softplus) delta = softplus_f32(delta);
+  float y = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kMaxPerLane; ++j)
-      if (lane + j * lanes < states) state[lane + j * lanes] = h[j];
+  for (int i = 0; i < kStates; ++i) {
+    h[i] = fmaf(ex2(delta * rate[i] * kLog2E), h[i], delta * x * b[i]);
+    y = fmaf(c[i], h[i], y);
+  }
+  if (live && left > 0) store_row<kVec>(state, left, h);
+  for (int o = lanes >> 1; o; o >>= 1) y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
+  if (a.D) y = fmaf(a.D[dd], x, y);
+  if (a.z) y *= silu_f32(z);
+  if (live && lane == 0) static_cast<T*>(a.out)[seq * static_cast<int64_t>(a.ld_out) + dd] = from_f32<T>(y);
 }
 
 // ---- tiled scan
@@ -311,37 +333,6 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ float ex2(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float rcp(float v) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
-constexpr float kLog2E = 1.44269504088896341f;
-
-// softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) <= 1, with log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1/3,
-// by its series 2 (s + s^3/3 + s^5/5 + ...): the first term left out is below 2^-25 of the sum. Exact to a few
-// steps for all v, where log(1 + e) rounded first would lose small e. Two special-function operations.
-__device__ __forceinline__ float softplus_fast(float v) {
-  const float e = ex2(-fabsf(v) * kLog2E);
-  const float s = e * rcp(2.0f + e), q = s * s;
-  float p = 1.0f / 15.0f;
-  p = fmaf(p, q, 1.0f / 13.0f);
-  p = fmaf(p, q, 1.0f / 11.0f);
-  p = fmaf(p, q, 1.0f / 9.0f);
-  p = fmaf(p, q, 1.0f / 7.0f);
-  p = fmaf(p, q, 1.0f / 5.0f);
-  p = fmaf(p, q, 1.0f / 3.0f);
-  const float l = fmaf(s * q, p, s);
-  return fmaf(2.0f, l, fmaxf(v, 0.0f));
-}
-__device__ __forceinline__ float silu_fast(float v) { return v * rcp(1.0f + ex2(-v * kLog2E)); }
-
 // Sums v[i] over groups of kLanes neighbouring lanes for kSteps values at once: lane l of a group ends with the sum
 // of value l % kSteps. Each exchange halves the values a lane holds, so kSteps sums take kSteps - 1 shuffles (and
 // one for every doubling of kLanes over kSteps) instead of kSteps * log2(kLanes).
@@ -606,7 +597,7 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
 #pragma unroll
       for (int i = 0; i < kOwn; ++i)
 #pragma unroll
-        for (int v = 0; v < V; ++v) delta[i][v] = softplus_fast(delta[i][v]);
+        for (int v = 0; v < V; ++v) delta[i][v] = softplus_f32(delta[i][v]);
     }
     if (left < kTile) {  // behind the sequence's end: a decay of 1 and no input, also where x is not finite
 #pragma unroll
@@ -663,7 +654,7 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
       for (int v = 0; v < V; ++v) y[v] = fmaf(skip[v], to_f32(rx.v[v]), p.v[v]);
       if (gate)
 #pragma unroll
-        for (int v = 0; v < V; ++v) y[v] *= silu_fast(to_f32(rz.v[v]));
+        for (int v = 0; v < V; ++v) y[v] *= silu_f32(to_f32(rz.v[v]));
       if (mine) store_row<S::kVec>(po + static_cast<int64_t>(t0 + t) * ldo, V, y);
     }
   };
@@ -732,15 +723,27 @@ cudaError_t scan_type(const mmfree_cuda_ssm_args& a, int sms, cudaStream_t s) {
   return fits(4 / sizeof(T)) ? scan_states<T, 4>(a, sms, s) : scan_states<T, 0>(a, sms, s);
 }
 
-cudaError_t step_any(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
+template <typename T>
+cudaError_t step_type(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
+  const int states = static_cast<int>(a.states), per = states <= 128 ? 4 : 8;
   int lanes = 1;
-  while (lanes < 32 && lanes < static_cast<int>(a.states)) lanes *= 2;
-  const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.channels) * lanes, 128)), static_cast<unsigned>(a.seqs));
+  while (lanes * per < states) lanes *= 2;
+  const auto one = [](const void* p, size_t pitch, size_t bytes) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && pitch * sizeof(T) % bytes == 0;
+  };
+  const size_t bytes = per * sizeof(T) < 16 ? per * sizeof(T) : 16;
+  const bool vec = states % per == 0 && aligned16(a.state) && aligned16(a.A) && one(a.B, a.ldb, bytes) && one(a.C, a.ldc, bytes);
+  const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.channels) * lanes, 256)), static_cast<unsigned>(a.seqs));
+  if (per == 4) return vec ? launch_k(step_kernel<T, 4, true>, grid, dim3(256), 0, s, false, a, lanes) : launch_k(step_kernel<T, 4, false>, grid, dim3(256), 0, s, false, a, lanes);
+  return vec ? launch_k(step_kernel<T, 8, true>, grid, dim3(256), 0, s, false, a, lanes) : launch_k(step_kernel<T, 8, false>, grid, dim3(256), 0, s, false, a, lanes);
+}
+
+cudaError_t step_any(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
   mark_device();
   switch (a.type) {
-    case MMFREE_T_F32: return launch_k(ssm_kernel<float>, grid, dim3(128), 0, s, false, a, lanes, true);
-    case MMFREE_T_BF16: return launch_k(ssm_kernel<__nv_bfloat16>, grid, dim3(128), 0, s, false, a, lanes, true);
-    default: return launch_k(ssm_kernel<__half>, grid, dim3(128), 0, s, false, a, lanes, true);
+    case MMFREE_T_F32: return step_type<float>(a, s);
+    case MMFREE_T_BF16: return step_type<__nv_bfloat16>(a, s);
+    default: return step_type<__half>(a, s);
   }
 }
 
