@@ -44,39 +44,37 @@ __device__ __forceinline__ void fetch8(const T* p, int n, Words<T, kCols>& w) {
   }
 }
 
-// A CTA holds a row in registers, kChunks chunks of 8 columns a thread, and walks the rows with a fixed stride; up to
-// two chunks it also keeps the weights, and loads the next row while this one is reduced and stored.
+// A CTA holds a row in registers, kChunks chunks of 8 columns a thread, and walks the rows with a fixed stride. Small
+// CTAs, several an SM, cover each other's reductions: 8192 rows of 6912 bf16 columns took 80 us with 864 threads of one
+// chunk and SMALL_US us with 216 of four. Short rows also keep the weights, and the next row is loaded while this one is
+// reduced and stored.
 template <typename T, typename Code, int kChunks, bool kVec>
-__global__ void __launch_bounds__(kChunks == 1 ? 256 : kChunks == 2 ? 512 : 1024, 1) norm_quant_kernel(NormQuantArgs a) {
-  constexpr bool kAhead = kChunks <= 2;
+__global__ void __launch_bounds__(kChunks == 8 ? 896 : 128 * kChunks, kChunks == 8 ? 1 : 8 / kChunks) norm_quant_kernel(NormQuantArgs a) {
+  constexpr bool kAhead = kChunks * sizeof(T) <= 4, kKeep = kChunks == 1;
   constexpr bool kS8 = std::is_same<Code, int8_t>::value;
   constexpr float kLimit = kS8 ? 127.0f : 448.0f;
   __shared__ float s_sum[2][32];
   __shared__ uint32_t s_most[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5;
   const bool add = a.residual != nullptr;
-  Words<T, kCols> next_x[kChunks], next_r[kChunks];
+  Words<T, kCols> next_x[kAhead ? kChunks : 1], next_r[kAhead ? kChunks : 1];
+  const auto fetch1 = [&](int64_t row, int c, int to) {
+    const int col = (tid + c * static_cast<int>(blockDim.x)) * kCols, n = a.cols - col;
+    if (n <= 0) return;
+    fetch8<T, kVec>(static_cast<const T*>(a.x) + row * a.ldx + col, n, next_x[to]);
+    if (add) fetch8<T, kVec>(static_cast<const T*>(a.residual) + row * a.ldr + col, n, next_r[to]);
+  };
   const auto fetch = [&](int64_t row) {
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const int col = (tid + c * static_cast<int>(blockDim.x)) * kCols, n = a.cols - col;
-      if (n <= 0) break;
-      fetch8<T, kVec>(static_cast<const T*>(a.x) + row * a.ldx + col, n, next_x[c]);
-      if (add) fetch8<T, kVec>(static_cast<const T*>(a.residual) + row * a.ldr + col, n, next_r[c]);
-    }
+    for (int c = 0; c < kChunks; ++c) fetch1(row, c, c);
   };
-  float w[kAhead ? kChunks : 1][kCols];
-  if constexpr (kAhead) {
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const int col = (tid + c * static_cast<int>(blockDim.x)) * kCols;
-      if (col < a.cols) load_row<kVec>(a.weight + col, a.cols - col, w[c]);
-    }
-    fetch(blockIdx.x);
+  float w[kCols];
+  if constexpr (kKeep) {
+    if (tid * kCols < a.cols) load_row<kVec>(a.weight + tid * kCols, a.cols - tid * kCols, w);
   }
+  if constexpr (kAhead) fetch(blockIdx.x);
   int buf = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, buf ^= 1) {
-    if constexpr (!kAhead) fetch(row);
     float t[kChunks][kCols], sum = 0.0f;
     uint32_t most[kChunks];  // |t| as its bits: ordered like the values, a NaN above all
 #pragma unroll
@@ -84,22 +82,26 @@ __global__ void __launch_bounds__(kChunks == 1 ? 256 : kChunks == 2 ? 512 : 1024
       const int col = (tid + c * static_cast<int>(blockDim.x)) * kCols, n = a.cols - col;
       most[c] = 0;
       if (n <= 0) continue;
+      constexpr bool kNow = !kAhead;
+      const int from = kNow ? 0 : c;
+      if constexpr (kNow) fetch1(row, c, 0);
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) t[c][i] = next_x[c][i];
+      for (int i = 0; i < kCols; ++i) t[c][i] = next_x[from][i];
       if (add) {
 #pragma unroll
-        for (int i = 0; i < kCols; ++i) t[c][i] = to_f32(from_f32<T>(next_r[c][i] + t[c][i]));
+        for (int i = 0; i < kCols; ++i) t[c][i] = to_f32(from_f32<T>(next_r[from][i] + t[c][i]));
         store_row<kVec>(static_cast<T*>(a.residual) + row * a.ldr + col, n, t[c]);
       }
-      if constexpr (!kAhead) load_row<kVec>(a.weight + col, n, w[0]);
+      if constexpr (!kKeep) load_row<kVec>(a.weight + col, n, w);
 #pragma unroll
       for (int i = 0; i < kCols; ++i) {
         sum = fmaf(t[c][i], t[c][i], sum);
-        t[c][i] = __fmul_rn(t[c][i], w[kAhead ? c : 0][i]);
+        t[c][i] = __fmul_rn(t[c][i], w[i]);
         most[c] = max(most[c], __float_as_uint(t[c][i]) & 0x7FFFFFFFu);
       }
     }
-    if (kAhead && row + gridDim.x < a.rows) fetch(row + gridDim.x);
+    if constexpr (kAhead)
+      if (row + gridDim.x < a.rows) fetch(row + gridDim.x);
     uint32_t row_most = 0;
     if (a.group == 0) {
 #pragma unroll
@@ -191,7 +193,7 @@ template <typename T, typename Code, bool kVec>
 cudaError_t launch_cols(const NormQuantArgs& a, cudaStream_t s) {
   const int chunks = static_cast<int>(ceil_div(a.cols, kCols));
   // a thread holds 1 to 8 chunks of the row in registers
-  const int per = chunks <= 256 ? 1 : chunks <= 1024 ? 2 : chunks <= 4096 ? 4 : 8;
+  const int per = chunks <= 128 ? 1 : chunks <= 512 ? 2 : chunks <= 2048 ? 4 : 8;
   const int threads = static_cast<int>(ceil_div(ceil_div(chunks, per), 32) * 32);
   switch (per) {
     case 1: return launch_chunks<T, Code, 1, kVec>(a, threads, s);

@@ -61,28 +61,18 @@ __device__ __forceinline__ void conv_load_taps(const mmfree_cuda_conv_args& a, i
   for (int i = 0; i < V; ++i) bias[i] = a.bias ? a.bias[d + i] : 0.0f;
 }
 
-// in: the window's W - 1 older inputs, then the newest; returns the output of each channel.
+// The output of each channel for the newest input in[W - 1]; in[0] to in[W - 2] are the older ones.
 template <int W, int V>
-__device__ __forceinline__ void conv_token(const float (&win)[W - 1][V], const float (&x)[V], const float (&w)[V][W],
-                                           const float (&bias)[V], bool silu, float (&y)[V]) {
+__device__ __forceinline__ void conv_token(const float (*in)[V], const float (&w)[V][W], const float (&bias)[V], bool silu, float (&y)[V]) {
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    float s = bias[i];
+    y[i] = bias[i];
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) s = fmaf(w[i][j], win[j][i], s);
-    s = fmaf(w[i][W - 1], x[i], s);
-    y[i] = silu ? silu_f32(s) : s;
+    for (int j = 0; j < W; ++j) y[i] = fmaf(w[i][j], in[j][i], y[i]);
   }
-}
-
-template <int W, int V>
-__device__ __forceinline__ void conv_shift(float (&win)[W - 1][V], const float (&x)[V]) {
+  if (silu)
 #pragma unroll
-  for (int j = 0; j + 1 < W - 1; ++j)
-#pragma unroll
-    for (int i = 0; i < V; ++i) win[j][i] = win[j + 1][i];
-#pragma unroll
-  for (int i = 0; i < V; ++i) win[W - 2][i] = x[i];
+    for (int i = 0; i < V; ++i) y[i] = silu_f32(y[i]);
 }
 
 // A CTA owns a tile of `rows` tokens for a block of channels. The tile in which a sequence
@@ -161,22 +151,39 @@ __global__ void __launch_bounds__(128) conv_kernel(mmfree_cuda_conv_args a, int 
 #pragma unroll
       for (int j = 0; j < W - 1; ++j) load_row<kVec>(x + (t - (W - 1) + j) * ldx, V, win[j]);
     }
-    // eight tokens' loads in flight together (those behind the last read it again)
+    // eight tokens' loads in flight together
     constexpr int kBatch = 8;
-    for (; t < stop; t += kBatch) {
+    float in[W - 1 + kBatch][V];
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) in[j][i] = win[j][i];
+    for (; t + kBatch <= stop; t += kBatch) {
       Words<T, V> raw[kBatch];
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) raw[k].load(x + min(t + k, stop - 1) * ldx);
+      for (int k = 0; k < kBatch; ++k) raw[k].load(x + (t + k) * ldx);
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
-        if (t + k >= stop) break;
-        float v[V], y[V];
+        float y[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = raw[k][i];
-        conv_token<W, V>(win, v, w, bias, silu, y);
+        for (int i = 0; i < V; ++i) in[W - 1 + k][i] = raw[k][i];
+        conv_token<W, V>(in + k, w, bias, silu, y);
         store_row<kVec>(out + (t + k) * ldo, V, y);
-        conv_shift<W, V>(win, v);
       }
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) in[j][i] = in[kBatch + j][i];
+    }
+    for (; t < stop; ++t) {
+      float y[V];
+      load_row<kVec>(x + t * ldx, V, in[W - 1]);
+      conv_token<W, V>(in, w, bias, silu, y);
+      store_row<kVec>(out + t * ldo, V, y);
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) in[j][i] = in[j + 1][i];
     }
   }
 }
@@ -190,22 +197,21 @@ __global__ void __launch_bounds__(128) conv_step_kernel(mmfree_cuda_conv_args a)
   if (slot < 0) return;
   const int64_t pitch = static_cast<int64_t>(a.channels);
   T* st = a.state ? static_cast<T*>(a.state) + (slot * (W - 1)) * pitch + d : nullptr;
-  float win[W - 1][V], v[V], y[V], w[V][W], bias[V];
-  load_row<kVec>(static_cast<const T*>(a.x) + s * static_cast<int64_t>(a.ldx) + d, V, v);
+  float in[W][V], y[V], w[V][W], bias[V];
+  load_row<kVec>(static_cast<const T*>(a.x) + s * static_cast<int64_t>(a.ldx) + d, V, in[W - 1]);
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) {
-    if (st) load_row<kVec>(st + j * pitch, V, win[j]);
+    if (st) load_row<kVec>(st + j * pitch, V, in[j]);
     else
 #pragma unroll
-      for (int i = 0; i < V; ++i) win[j][i] = 0.0f;
+      for (int i = 0; i < V; ++i) in[j][i] = 0.0f;
   }
   conv_load_taps<W, V>(a, d, w, bias);
-  conv_token<W, V>(win, v, w, bias, a.silu != 0, y);
+  conv_token<W, V>(in, w, bias, a.silu != 0, y);
   store_row<kVec>(static_cast<T*>(a.out) + s * static_cast<int64_t>(a.ld_out) + d, V, y);
-  conv_shift<W, V>(win, v);
   if (st)
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) store_row<kVec>(st + j * pitch, V, win[j]);
+    for (int j = 0; j < W - 1; ++j) store_row<kVec>(st + j * pitch, V, in[j + 1]);
 }
 
 template <typename T, int W, int V>
@@ -270,47 +276,74 @@ __device__ __forceinline__ float softplus_f32(float v) {
   return fmaf(2.0f, l, fmaxf(v, 0.0f));
 }
 
-// One token of a stream: `lanes` lanes (a power of two) a channel, kStates neighbouring states a lane, kVec: read and
-// written by 16 bytes. Bound by the state's bytes; every lane repeats its channel's softplus and gate, which costs less
-// than passing them on.
-template <typename T, int kStates, bool kVec>
+// One token of each of kStreams streams: `lanes` lanes (a power of two) a channel, kStates neighbouring states a lane,
+// kVec: read and written by 16 bytes. Bound by the state's bytes, which have to be in flight together: four streams a
+// thread where there are enough. Every lane repeats its channel's softplus and gate, which costs less than passing
+// them on.
+template <typename T, int kStates, int kStreams, bool kVec>
 __global__ void __launch_bounds__(256) step_kernel(mmfree_cuda_ssm_args a, int lanes) {
-  const int64_t channels = static_cast<int64_t>(a.channels);
+  const int64_t channels = static_cast<int64_t>(a.channels), seqs = static_cast<int64_t>(a.seqs);
   const int states = static_cast<int>(a.states), lane = threadIdx.x & (lanes - 1);
-  const int64_t d = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes, seq = blockIdx.y;
-  const int64_t slot = sequence_slot(a.slots, static_cast<int64_t>(a.slot_count), seq);
-  if (slot < 0) return;
+  const int64_t d = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes, seq0 = static_cast<int64_t>(blockIdx.y) * kStreams;
   const bool live = d < channels;
   const int64_t dd = live ? d : channels - 1;
   const int n = lane * kStates, left = states - n;
-  float* const state = a.state + (slot * channels + dd) * states + n;
-  const float* const rates = a.A + dd * states + n;
   const int64_t group = dd / (channels / static_cast<int64_t>(a.groups));
-  const T* const B = static_cast<const T*>(a.B) + seq * static_cast<int64_t>(a.ldb) + group * states + n;
-  const T* const C = static_cast<const T*>(a.C) + seq * static_cast<int64_t>(a.ldc) + group * states + n;
-  float h[kStates] = {}, rate[kStates] = {}, b[kStates] = {}, c[kStates] = {};
-  if (left > 0) {
-    load_row<kVec>(state, left, h);
-    load_row<kVec>(rates, left, rate);
-    load_row<kVec>(B, left, b);
-    load_row<kVec>(C, left, c);
-  }
-  const float x = to_f32(static_cast<const T*>(a.x)[seq * static_cast<int64_t>(a.ldx) + dd]);
-  float delta = to_f32(static_cast<const T*>(a.dt)[seq * static_cast<int64_t>(a.ld_dt) + dd]);
-  const float z = a.z ? to_f32(static_cast<const T*>(a.z)[seq * static_cast<int64_t>(a.ldz) + dd]) : 0.0f;
-  if (a.dt_bias) delta += a.dt_bias[dd];
-  if (a.dt_softplus) delta = softplus_f32(delta);
-  float y = 0.0f;
+  // all streams' loads without a branch or a use between them: an absent stream reads another one's
+  bool there[kStreams];
+  float* state[kStreams];
+  float h[kStreams][kStates], rate[kStates] = {};
+  Words<T, kVec ? kStates : 1> b[kStreams][kVec ? 1 : kStates], c[kStreams][kVec ? 1 : kStates];
+  Words<T, 1> x[kStreams], delta[kStreams], z[kStreams];
 #pragma unroll
-  for (int i = 0; i < kStates; ++i) {
-    h[i] = fmaf(ex2(delta * rate[i] * kLog2E), h[i], delta * x * b[i]);
-    y = fmaf(c[i], h[i], y);
+  for (int k = 0; k < kStreams; ++k) {
+    const int64_t seq = min(seq0 + k, seqs - 1), slot = sequence_slot(a.slots, static_cast<int64_t>(a.slot_count), seq);
+    there[k] = slot >= 0 && seq0 + k < seqs;
+    state[k] = a.state + (max(slot, int64_t(0)) * channels + dd) * states + min(n, states - 1);
   }
-  if (live && left > 0) store_row<kVec>(state, left, h);
-  for (int o = lanes >> 1; o; o >>= 1) y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
-  if (a.D) y = fmaf(a.D[dd], x, y);
-  if (a.z) y *= silu_f32(z);
-  if (live && lane == 0) static_cast<T*>(a.out)[seq * static_cast<int64_t>(a.ld_out) + dd] = from_f32<T>(y);
+#pragma unroll
+  for (int k = 0; k < kStreams; ++k) {
+    const int64_t seq = min(seq0 + k, seqs - 1);
+    const T* const pb = static_cast<const T*>(a.B) + seq * static_cast<int64_t>(a.ldb) + group * states;
+    const T* const pc = static_cast<const T*>(a.C) + seq * static_cast<int64_t>(a.ldc) + group * states;
+    if constexpr (kVec) {  // a lane behind the last state reads that one's, and stores nothing
+      const int at = min(n, states - kStates);
+      load_row<true>(state[k] + (at - min(n, states - 1)), kStates, h[k]);
+      b[k][0].load(pb + at);
+      c[k][0].load(pc + at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kStates; ++i) {
+        const int at = min(n + i, states - 1);
+        h[k][i] = state[k][at - min(n, states - 1)];
+        b[k][i].load(pb + at);
+        c[k][i].load(pc + at);
+      }
+    }
+    x[k].load(static_cast<const T*>(a.x) + seq * static_cast<int64_t>(a.ldx) + dd);
+    delta[k].load(static_cast<const T*>(a.dt) + seq * static_cast<int64_t>(a.ld_dt) + dd);
+    if (a.z) z[k].load(static_cast<const T*>(a.z) + seq * static_cast<int64_t>(a.ldz) + dd);
+  }
+  if (left > 0) load_row<kVec>(a.A + dd * states + n, left, rate);
+  const float bias = a.dt_bias ? a.dt_bias[dd] : 0.0f, skip = a.D ? a.D[dd] : 0.0f;
+#pragma unroll
+  for (int k = 0; k < kStreams; ++k) {
+    const float xk = x[k][0];
+    float dl = delta[k][0] + bias, y = 0.0f;
+    if (a.dt_softplus) dl = softplus_f32(dl);
+#pragma unroll
+    for (int i = 0; i < kStates; ++i) {
+      const float bi = kVec ? b[k][0][kVec ? i : 0] : b[k][kVec ? 0 : i][0], ci = kVec ? c[k][0][kVec ? i : 0] : c[k][kVec ? 0 : i][0];
+      h[k][i] = fmaf(ex2(dl * rate[i] * kLog2E), h[k][i], dl * xk * bi);
+      if (i < left) y = fmaf(ci, h[k][i], y);
+    }
+    for (int o = lanes >> 1; o; o >>= 1) y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
+    if (!live || !there[k]) continue;
+    if (left > 0) store_row<kVec>(state[k], left, h[k]);
+    y = fmaf(skip, xk, y);
+    if (a.z) y *= silu_f32(z[k][0]);
+    if (lane == 0) static_cast<T*>(a.out)[(seq0 + k) * static_cast<int64_t>(a.ld_out) + dd] = from_f32<T>(y);
+  }
 }
 
 // ---- tiled scan
@@ -723,6 +756,15 @@ cudaError_t scan_type(const mmfree_cuda_ssm_args& a, int sms, cudaStream_t s) {
   return fits(4 / sizeof(T)) ? scan_states<T, 4>(a, sms, s) : scan_states<T, 0>(a, sms, s);
 }
 
+template <typename T, int kStates, bool kVec>
+cudaError_t step_launch(const mmfree_cuda_ssm_args& a, int lanes, cudaStream_t s) {
+  const unsigned blocks = static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.channels) * lanes, 256));
+  // four streams a thread where one stream a thread would be more threads than the SMs hold at once
+  if (static_cast<int64_t>(blocks) * static_cast<int64_t>(a.seqs) > 148 * 8)
+    return launch_k(step_kernel<T, kStates, 4, kVec>, dim3(blocks, static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.seqs), 4))), dim3(256), 0, s, false, a, lanes);
+  return launch_k(step_kernel<T, kStates, 1, kVec>, dim3(blocks, static_cast<unsigned>(a.seqs)), dim3(256), 0, s, false, a, lanes);
+}
+
 template <typename T>
 cudaError_t step_type(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
   const int states = static_cast<int>(a.states), per = states <= 128 ? 4 : 8;
@@ -733,9 +775,8 @@ cudaError_t step_type(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
   };
   const size_t bytes = per * sizeof(T) < 16 ? per * sizeof(T) : 16;
   const bool vec = states % per == 0 && aligned16(a.state) && aligned16(a.A) && one(a.B, a.ldb, bytes) && one(a.C, a.ldc, bytes);
-  const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.channels) * lanes, 256)), static_cast<unsigned>(a.seqs));
-  if (per == 4) return vec ? launch_k(step_kernel<T, 4, true>, grid, dim3(256), 0, s, false, a, lanes) : launch_k(step_kernel<T, 4, false>, grid, dim3(256), 0, s, false, a, lanes);
-  return vec ? launch_k(step_kernel<T, 8, true>, grid, dim3(256), 0, s, false, a, lanes) : launch_k(step_kernel<T, 8, false>, grid, dim3(256), 0, s, false, a, lanes);
+  if (per == 4) return vec ? step_launch<T, 4, true>(a, lanes, s) : step_launch<T, 4, false>(a, lanes, s);
+  return vec ? step_launch<T, 8, true>(a, lanes, s) : step_launch<T, 8, false>(a, lanes, s);
 }
 
 cudaError_t step_any(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
