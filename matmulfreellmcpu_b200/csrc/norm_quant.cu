@@ -53,20 +53,28 @@ __global__ void __launch_bounds__(kChunks == 8 ? 896 : 128 * kChunks, kChunks ==
   constexpr bool kAhead = kChunks * sizeof(T) <= 4, kKeep = kChunks == 1;
   constexpr bool kS8 = std::is_same<Code, int8_t>::value;
   constexpr float kLimit = kS8 ? 127.0f : 448.0f;
-  __shared__ float s_sum[2][32];
-  __shared__ uint32_t s_most[2][32];
+  __shared__ __align__(16) float s_sum[2][32];
+  __shared__ __align__(16) uint32_t s_most[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5;
   const bool add = a.residual != nullptr;
-  Words<T, kCols> next_x[kAhead ? kChunks : 1], next_r[kAhead ? kChunks : 1];
-  const auto fetch1 = [&](int64_t row, int c, int to) {
-    const int col = (tid + c * static_cast<int>(blockDim.x)) * kCols, n = a.cols - col;
-    if (n <= 0) return;
-    fetch8<T, kVec>(static_cast<const T*>(a.x) + row * a.ldx + col, n, next_x[to]);
-    if (add) fetch8<T, kVec>(static_cast<const T*>(a.residual) + row * a.ldr + col, n, next_r[to]);
-  };
+  const int parts_shift = a.group ? __ffs(a.group) - 1 : 0;
+  const float inv_cols = 1.0f / static_cast<float>(a.cols);
+  Words<T, kCols> next_x[kChunks], next_r[kChunks];
   const auto fetch = [&](int64_t row) {
+    const T* const px = static_cast<const T*>(a.x) + row * a.ldx;
+    const T* const pr = static_cast<const T*>(a.residual) + (add ? row * a.ldr : 0);
+    // whole chunks without a branch between the loads: a thread behind the row's end reads its last chunk
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) fetch1(row, c, c);
+    for (int c = 0; c < kChunks; ++c) {
+      const int at = (tid + c * static_cast<int>(blockDim.x)) * kCols, col = kVec ? min(at, a.cols - kCols) : at;
+      fetch8<T, kVec>(px + col, a.cols - col, next_x[c]);
+    }
+    if (add)
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const int at = (tid + c * static_cast<int>(blockDim.x)) * kCols, col = kVec ? min(at, a.cols - kCols) : at;
+        fetch8<T, kVec>(pr + col, a.cols - col, next_r[c]);
+      }
   };
   float w[kCols];
   if constexpr (kKeep) {
@@ -75,6 +83,7 @@ __global__ void __launch_bounds__(kChunks == 8 ? 896 : 128 * kChunks, kChunks ==
   if constexpr (kAhead) fetch(blockIdx.x);
   int buf = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, buf ^= 1) {
+    if constexpr (!kAhead) fetch(row);
     float t[kChunks][kCols], sum = 0.0f;
     uint32_t most[kChunks];  // |t| as its bits: ordered like the values, a NaN above all
 #pragma unroll
@@ -82,14 +91,11 @@ __global__ void __launch_bounds__(kChunks == 8 ? 896 : 128 * kChunks, kChunks ==
       const int col = (tid + c * static_cast<int>(blockDim.x)) * kCols, n = a.cols - col;
       most[c] = 0;
       if (n <= 0) continue;
-      constexpr bool kNow = !kAhead;
-      const int from = kNow ? 0 : c;
-      if constexpr (kNow) fetch1(row, c, 0);
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) t[c][i] = next_x[from][i];
+      for (int i = 0; i < kCols; ++i) t[c][i] = next_x[c][i];
       if (add) {
 #pragma unroll
-        for (int i = 0; i < kCols; ++i) t[c][i] = to_f32(from_f32<T>(next_r[from][i] + t[c][i]));
+        for (int i = 0; i < kCols; ++i) t[c][i] = to_f32(from_f32<T>(next_r[c][i] + t[c][i]));
         store_row<kVec>(static_cast<T*>(a.residual) + row * a.ldr + col, n, t[c]);
       }
       if constexpr (!kKeep) load_row<kVec>(a.weight + col, n, w);
@@ -125,21 +131,23 @@ __global__ void __launch_bounds__(kChunks == 8 ? 896 : 128 * kChunks, kChunks ==
         s_most[buf][tid >> 5] = row_most;
       }
       __syncthreads();  // one a row: the next row's partials go to the other half
-      // every warp sums all partials in the same order
-      sum = lane < warps ? s_sum[buf][lane] : 0.0f;
-      row_most = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? s_most[buf][lane] : 0u);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+      // every thread sums the warps' partials, in the same order
+      sum = 0.0f;
+      for (int i = 0; i < warps; ++i) sum += s_sum[buf][i];
+      if (a.group == 0) {
+        row_most = 0;
+        for (int i = 0; i < warps; ++i) row_most = max(row_most, s_most[buf][i]);
+      }
     }
-    const float rstd = 1.0f / sqrtf(sum / static_cast<float>(a.cols) + a.eps);
+    const float rstd = rsqrtf(fmaf(sum, inv_cols, a.eps));
     float* const scales = a.scales + row * a.parts;
-    if (a.group == 0 && tid == 0) scales[0] = __uint_as_float(row_most) * rstd / kLimit;
+    if (a.group == 0 && tid == 0) scales[0] = __uint_as_float(row_most) * rstd * (1.0f / kLimit);
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       const int col = (tid + c * static_cast<int>(blockDim.x)) * kCols, n = a.cols - col;
       if (n <= 0) continue;
       const float m = __uint_as_float(a.group ? most[c] : row_most);
-      if (a.group && (col & (a.group - 1)) == 0) scales[col / a.group] = m * rstd / kLimit;
+      if (a.group && (col & (a.group - 1)) == 0) scales[col >> parts_shift] = m * rstd * (1.0f / kLimit);
       const float inv = kLimit / m;
       Pack<uint8_t, kCols> q;
       if constexpr (kS8) {
