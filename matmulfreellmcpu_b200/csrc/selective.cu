@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
       Pack<float, VB> vb, vc;
 #pragma unroll
       for (int v = 0; v < VB; ++v) {
-        vb.v[v] = n < states ? to_f32(rb.v[v]) : 0.0f;
+        vb.v[v] = n < states && at / kN < left ? to_f32(rb.v[v]) : 0.0f;  // 0 behind the end too: 0 * inf is not 0
         vc.v[v] = n < states ? to_f32(rc.v[v]) : 0.0f;
       }
       *reinterpret_cast<Pack<float, VB>*>(&sh.b[buf][at / kN][n]) = vb;

@@ -340,6 +340,27 @@ def test_selective_scan_extreme_steps(cuda):
     close(state, new, nbound, "state")
 
 
+def test_selective_scan_nonfinite_values_stay_where_they_are(cuda):
+    """An infinity in a sequence's last token, and NaN in rows and sequences around it."""
+    p = ssm_inputs(40, 64, 16, 1, "fp32", 21, 3)
+    starts, slots = [2, 11, 11, 37], torch.tensor([0, 1, 2], dtype=torch.int32)
+    for k in ("x", "dt", "B", "C", "z"):
+        p[k][:2] = torch.nan   # rows in front of the first and behind the last sequence
+        p[k][37:] = torch.nan
+    p["B"][10, 0, 3] = torch.inf
+    p["x"][10] = p["x"][10].abs() + 0.1
+    clean = {k: v.clone() for k, v in p.items()}
+    clean["B"][10, 0, 3] = 1.0
+    want, bound, new, nbound = R.ssm_ref(clean["x"], clean["dt"], clean["A"], clean["B"], clean["C"], clean["D"], clean["z"],
+                                         clean["dt_bias"], True, clean["state"], starts, slots, pieces=16)
+    out, state = run_ssm(cuda, p, starts, slots, 0)
+    rows = [t for t in range(2, 37) if t != 10]
+    close(out[rows], want[rows], bound[rows], "y")
+    assert torch.isinf(state[0, :, 3]).all()
+    keep = [n for n in range(16) if n != 3]
+    close(state[:, :, keep], new[:, :, keep], nbound[:, :, keep], "state")
+
+
 @pytest.mark.parametrize("kind", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("streams,channels,states,groups", [(1, 2048, 16, 1), (5, 33, 16, 1), (3, 48, 5, 2), (2, 40, 128, 4),
                                                             (4, 12, 64, 1), (2, 3, 256, 1), (64, 256, 16, 1), (3, 8, 1, 1)])
@@ -499,6 +520,38 @@ def test_another_stream(cuda):
     got = api.causal_conv(x, w, silu=True, stream=side)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(got, want)
+
+
+def test_large_calls_in_a_captured_graph(cuda):
+    """Calls of many rows and tokens ask the device for its size; that is allowed in a capture."""
+    x = torch.randn(600, 512, device=cuda)
+    res, w = torch.randn(600, 512, device=cuda), torch.ones(512, device=cuda)
+    p = {k: v.to(cuda) for k, v in ssm_inputs(600, 512, 16, 1, "fp32", 5, 1).items()}
+    codes, scales = torch.randint(0, 256, (300, 256), dtype=torch.uint8, device=cuda), torch.rand(300, 4, device=cuda)
+
+    def run(res, st):
+        q, s = api.add_rmsnorm_quant(x, w, res)
+        m = api.int4_matvec(q, codes, scales, 128, x_scales=s)
+        return q, s, m, api.selective_scan(p["x"], p["dt"], p["A"], p["B"], p["C"], state=st)
+
+    r1, s1 = res.clone(), p["state"].clone()
+    want = run(r1, s1)
+    r2, s2 = res.clone(), p["state"].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(r2, s2)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((*want, r1, s1), (*got, r2, s2)))
+
+
+def test_inputs_that_require_gradients_are_refused(cuda):
+    x, w = torch.randn(4, 16, device=cuda), torch.randn(16, 4, device=cuda, requires_grad=True)
+    with pytest.raises(api.MmfreeError) as e:
+        api.causal_conv(x, w)
+    assert e.value.code == _lib.E_INVALID and "gradient" in str(e.value)
+    with torch.no_grad():
+        api.causal_conv(x, w)
 
 
 def test_repeated_calls_give_the_same_bits(cuda):
