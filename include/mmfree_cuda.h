@@ -213,8 +213,8 @@ int mmfree_cuda_add_rmsnorm_quant(void* codes, float* scales, const void* x, siz
 /* out[m, n] = x_scales[m] * sum_k x[m, k] * (u[n, k] - zero[n, k / group]) * scale[n, k / group]
  * for 4-bit weights u in 0..15. codes: [out_dim, ceil(in_dim / 2)] bytes with row pitch
  * ld_codes bytes, element 2j in the low and 2j + 1 in the high half of byte j; scales
- * [out_dim, ceil(in_dim / group)] of scale_type (F32, BF16 or F16) and zeros (uint8, same
- * shape; NULL: 8) contiguous; group a multiple of 32. x [rows, in_dim] of x_type: F32, BF16
+ * [out_dim, ceil(in_dim / group)] of scale_type (F32, BF16 or F16) and zeros (uint8 of at
+ * most 127, same shape; NULL: 8) contiguous; group a multiple of 32. x [rows, in_dim] of x_type: F32, BF16
  * or F16 with x_scales NULL, or S8 / E4M3 codes with the scales of
  * mmfree_cuda_add_rmsnorm_quant: x_scales [rows] with x_group 0, or [rows, ceil(in_dim /
  * group)] with x_group == group. out [rows, out_dim] contiguous of out_type (F32, BF16 or

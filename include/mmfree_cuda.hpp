@@ -151,5 +151,19 @@ inline void rmsnorm_swishgate(float* out, const float* g, const float* o, const 
   check(mmfree_cuda_rmsnorm_swishgate(out, g, o, weight, rows, cols, eps, stream));
 }
 
+// The operators of a block with a selective scan (mmfree_cuda.h describes the arguments).
+inline void causal_conv(const mmfree_cuda_conv_args& a, void* stream = nullptr) {
+  check(mmfree_cuda_causal_conv(&a, stream));
+}
+inline void causal_conv_step(const mmfree_cuda_conv_args& a, void* stream = nullptr) {
+  check(mmfree_cuda_causal_conv_step(&a, stream));
+}
+inline void selective_scan(const mmfree_cuda_ssm_args& a, void* stream = nullptr) {
+  check(mmfree_cuda_selective_scan(&a, stream));
+}
+inline void selective_step(const mmfree_cuda_ssm_args& a, void* stream = nullptr) {
+  check(mmfree_cuda_selective_step(&a, stream));
+}
+
 }  // namespace cuda
 }  // namespace mmfree
