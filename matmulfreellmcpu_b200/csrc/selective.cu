@@ -8,6 +8,7 @@
 #include "block_ops.h"
 #include "common.cuh"
 #include "elements.cuh"
+#include "tcgen05.cuh"
 
 #include <atomic>
 #include <type_traits>
@@ -409,6 +410,7 @@ struct ScanShape {
   static constexpr int kCtas = kCtas_;                          // CTAs an SM that the registers leave room for
   static constexpr int kBytes = kBytes_;                        // of an access: 16 or 4, copied asynchronously, or 0: one element
   static constexpr bool kVec = kBytes > 0;
+  static constexpr bool kMaySplit = kCtas < 4;                  // the shape for many CTAs is never short of them
   static constexpr int kN = kLanes * kStates;                   // states, padded
   static constexpr int kChannels = kScan / kLanes * kPer;
   static constexpr int kWide = kVec ? kBytes / sizeof(T) : 1;
@@ -426,6 +428,7 @@ struct ScanShape {
     float2 in[2][kTile][kChannels];  // delta, delta * x
     float y[2][kTile][kChannels];
     float b[2][kTile][kN], c[2][kTile][kN];
+    float carry[kPer * (kStates + 1)][kScan];  // a piece's last state and sum of deltas, for the pieces behind it
     Raw raw[kStages];
   };
 };
@@ -435,15 +438,20 @@ struct ScanShape {
 // once per token and channel, finishes and stores the previous tile's outputs, and keeps two more tiles in flight
 // from memory. They meet at one barrier a tile. In one half the jobs alternated, and each left the issue slots of
 // its latencies unused.
+// splits > 1: the CTAs of a cluster take a sequence's pieces. A state after a piece is the piece's own, from a state of
+// 0, plus the state before it times exp(A * the sum of the piece's deltas): so the pieces between the first and the last
+// run without outputs first, then every piece but the first starts from the states and sums of those before it, read
+// from their shared memory. Two passes for a sequence, each over 1 / splits of it.
 // What a turn of the recurrence reads from shared memory bounds it next to the special-function unit (128 bytes of
 // registers a clock): kPer channels a lane share one read of B and C.
 template <typename S>
-__global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(mmfree_cuda_ssm_args a, int blocks_per_group) {
+__global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(mmfree_cuda_ssm_args a, int blocks_per_group, int splits_asked) {
   using T = typename S::Type;
   constexpr int kLanes = S::kLanes, kStates = S::kStates, kPer = S::kPer, kTile = S::kTile, kN = S::kN, V = S::V, VB = S::VB;
   constexpr int kGroup = 4;                                  // tokens of a turn of the recurrence
   constexpr int kSteps = kLanes < kGroup ? kLanes : kGroup;  // tokens summed over lanes together
   constexpr int kPairs = kStates / 2;
+  const int splits = S::kMaySplit ? splits_asked : 1;
   static_assert(kTile % kGroup == 0 && sizeof(typename S::Shared) <= 227 * 1024, "tile shape");
   extern __shared__ __align__(16) char smem_raw[];
   auto& sh = *reinterpret_cast<typename S::Shared*>(smem_raw);
@@ -455,11 +463,23 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
   if (slot < 0) return;
   const int states = static_cast<int>(a.states);
   const int64_t channels = static_cast<int64_t>(a.channels), per_group = channels / static_cast<int64_t>(a.groups);
-  const int64_t group = blockIdx.x / blocks_per_group;
-  const int64_t first = (blockIdx.x - group * blocks_per_group) * S::kChannels;  // within the group
+  const int rank = splits > 1 ? blockIdx.x % splits : 0;
+  const int64_t block = blockIdx.x / splits, group = block / blocks_per_group;
+  const int64_t first = (block - group * blocks_per_group) * S::kChannels;  // within the group
   const int live = static_cast<int>(min(static_cast<int64_t>(S::kChannels), per_group - first));
   const int64_t base = group * per_group + first;
-  const int length = static_cast<int>(e - b), tiles = (length + kTile - 1) / kTile;
+  // this CTA's piece: at least four tiles, and three pieces or one (two would run one after the other)
+  int pieces = 1, length = static_cast<int>(e - b);
+  if (splits > 1) {
+    pieces = min(splits, length / (4 * kTile));
+    if (pieces < 3) pieces = 1;
+    const int piece = (length + pieces * kTile - 1) / (pieces * kTile) * kTile;
+    pieces = (length + piece - 1) / piece;
+    b += min(rank * piece, length);
+    length = max(0, min(piece, length - rank * piece));
+  }
+  const bool mine_first = rank == 0, between = rank > 0 && rank < pieces - 1, behind = rank > 0 && rank < pieces;
+  const int tiles = (length + kTile - 1) / kTile;
 
   if (threadIdx.x < S::kScan) {
     // ---- the recurrence
@@ -475,7 +495,7 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int n = lane * kStates + 2 * j + i;
-          hv[i] = n < states && pool ? pool[d * states + n] : 0.0f;
+          hv[i] = n < states && pool && mine_first ? pool[d * states + n] : 0.0f;
           rv[i] = n < states ? a.A[d * states + n] * kLog2E : 0.0f;
         }
         h[c][j] = pack2(hv[0], hv[1]);
@@ -484,8 +504,11 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
     }
     // the recurrence over `count` turns from token t0 of the tile; the outputs are stored behind the last one, since
     // a store between them would keep the next turn's loads from shared memory behind it
-    const auto turns = [&](int buf, int t0, auto count) {
+    double deltas[kPer] = {};
+    const auto turns = [&](int buf, int t0, auto count, auto outputs) {
       constexpr int kCount = decltype(count)::value;
+      constexpr bool kOut = decltype(outputs)::value;
+      float part_deltas[kPer] = {};
       float out[kCount][kPer][kGroup / kSteps];
 #pragma unroll
       for (int turn = 0; turn < kCount; ++turn) {
@@ -496,9 +519,10 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
           const Pack<float, 2 * kPer> in = *reinterpret_cast<const Pack<float, 2 * kPer>*>(&sh.in[buf][t][ch]);
           f32x2 bv[kPairs], cv[kPairs];
           *reinterpret_cast<Pack<float, kStates>*>(bv) = *reinterpret_cast<const Pack<float, kStates>*>(&sh.b[buf][t][lane * kStates]);
-          *reinterpret_cast<Pack<float, kStates>*>(cv) = *reinterpret_cast<const Pack<float, kStates>*>(&sh.c[buf][t][lane * kStates]);
+          if (kOut) *reinterpret_cast<Pack<float, kStates>*>(cv) = *reinterpret_cast<const Pack<float, kStates>*>(&sh.c[buf][t][lane * kStates]);
 #pragma unroll
           for (int c = 0; c < kPer; ++c) {
+            if (!kOut) part_deltas[c] += in.v[2 * c];
             const f32x2 dl = pack2(in.v[2 * c], in.v[2 * c]), dx = pack2(in.v[2 * c + 1], in.v[2 * c + 1]);
             f32x2 sum;
 #pragma unroll
@@ -506,13 +530,15 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
               float lo, hi;
               unpack2(mul2(dl, rate[c][j]), lo, hi);
               h[c][j] = fma2(pack2(ex2(lo), ex2(hi)), h[c][j], mul2(dx, bv[j]));
-              sum = j ? fma2(cv[j], h[c][j], sum) : mul2(cv[j], h[c][j]);
+              if (kOut) sum = j ? fma2(cv[j], h[c][j], sum) : mul2(cv[j], h[c][j]);
             }
+            if (!kOut) continue;
             float lo, hi;
             unpack2(sum, lo, hi);
             y[c][k] = lo + hi;
           }
         }
+        if (!kOut) continue;
 #pragma unroll
         for (int c = 0; c < kPer; ++c)
 #pragma unroll
@@ -523,7 +549,10 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
             out[turn][c][g / kSteps] = transpose_sum<kLanes, kSteps>(part, lane);
           }
       }
-      if (lane < kSteps)
+      if (!kOut) {
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) deltas[c] += part_deltas[c];  // over a piece in 64 bits
+      } else if (lane < kSteps)
 #pragma unroll
         for (int turn = 0; turn < kCount; ++turn)
 #pragma unroll
@@ -534,18 +563,57 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
             *reinterpret_cast<Pack<float, kPer>*>(&sh.y[buf][t0 + turn * kGroup + g + lane][ch]) = v;
           }
     };
-    __syncthreads();
     constexpr int kTurns = kTile / kGroup;
-    for (int tile = 0; tile < tiles; ++tile) {
-      const int buf = tile & 1, left = min(kTile, length - tile * kTile);
-      if (left > kTile - kGroup) {  // unrolled as a whole, so that loads and exponentials run ahead of the sums
-        turns(buf, 0, std::integral_constant<int, kTurns>{});
-      } else {
-#pragma unroll 1
-        for (int t = 0; t < left; t += 2 * kGroup) turns(buf, t, std::integral_constant<int, 2>{});
-      }
+    const auto sweep = [&](auto outputs) {
       __syncthreads();
+      for (int tile = 0; tile < tiles; ++tile) {
+        const int buf = tile & 1, left = min(kTile, length - tile * kTile);
+        if (left > kTile - kGroup) {  // unrolled as a whole, so that loads and exponentials run ahead of the sums
+          turns(buf, 0, std::integral_constant<int, kTurns>{}, outputs);
+        } else {
+#pragma unroll 1
+          for (int t = 0; t < left; t += 2 * kGroup) turns(buf, t, std::integral_constant<int, 2>{}, outputs);
+        }
+        __syncthreads();
+      }
+    };
+    if (between) sweep(std::false_type{});
+    // the first piece's outputs before the exchange, the others' behind it (one copy of the code for both)
+#pragma unroll 1
+    for (int phase = 0; phase < 2; ++phase) {
+      if (phase == 0 ? mine_first : behind) sweep(std::true_type{});
+      if (phase == 1 || splits == 1) break;
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) {
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j)
+          unpack2(h[c][j], sh.carry[c * (kStates + 1) + 2 * j][threadIdx.x], sh.carry[c * (kStates + 1) + 2 * j + 1][threadIdx.x]);
+        sh.carry[c * (kStates + 1) + kStates][threadIdx.x] = static_cast<float>(deltas[c]);
+      }
+      cluster_sync();
+      if (behind) {
+        const auto peer = [&](int value, int q) {
+          float v;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_map(smem_u32(&sh.carry[value][threadIdx.x]), q)) : "memory");
+          return v;
+        };
+        for (int q = 0; q < rank; ++q)
+#pragma unroll
+          for (int c = 0; c < kPer; ++c) {
+            const float sum = q ? peer(c * (kStates + 1) + kStates, q) : 0.0f;
+            const f32x2 sums = pack2(sum, sum);
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) {
+              const f32x2 end = pack2(peer(c * (kStates + 1) + 2 * j, q), peer(c * (kStates + 1) + 2 * j + 1, q));
+              float lo, hi;
+              unpack2(mul2(sums, rate[c][j]), lo, hi);
+              h[c][j] = q ? fma2(pack2(ex2(lo), ex2(hi)), h[c][j], end) : end;
+            }
+          }
+      }
     }
+    if (splits > 1) cluster_sync();  // before a CTA whose shared memory is read ends
+    if (rank != pieces - 1) return;
 #pragma unroll
     for (int c = 0; c < kPer; ++c) {
       if (!pool || ch + c >= live) break;
@@ -693,54 +761,78 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
   };
   // before the first half's tile 0: tile 0 prepared; in its tile t: t + 1 prepared, t - 1 finished, then its stage filled
   constexpr int kAhead = S::kStages - 1;
-  load(0);
-  if constexpr (S::kVec) {
-    load(1);
-    load(2);
-    copy_wait<kAhead - 1>();
-  }
-  prepare(0);
-  __syncthreads();
-  for (int tile = 0; tile < tiles; ++tile) {
-    if constexpr (S::kVec) copy_wait<kAhead - 2>();
-    else load(tile + 1);
-    prepare(tile + 1);
-    if (tile > 0) finish(tile - 1);
-    if constexpr (S::kVec) load(tile + kAhead);
+  const auto sweep = [&](bool outputs) {
+    load(0);
+    if constexpr (S::kVec) {
+      load(1);
+      load(2);
+      copy_wait<kAhead - 1>();
+    }
+    prepare(0);
     __syncthreads();
+    for (int tile = 0; tile < tiles; ++tile) {
+      if constexpr (S::kVec) copy_wait<kAhead - 2>();
+      else load(tile + 1);
+      prepare(tile + 1);
+      if (outputs && tile > 0) finish(tile - 1);
+      if constexpr (S::kVec) load(tile + kAhead);
+      __syncthreads();
+    }
+    if (outputs) finish(tiles - 1);
+  };
+#pragma unroll 1
+  for (int phase = 0; phase < 2; ++phase) {
+    if (phase == 0 ? mine_first || between : behind) sweep(phase == 1 || mine_first);
+    if (splits > 1) cluster_sync();
+    else break;
   }
-  finish(tiles - 1);
 }
 
 template <typename S>
-cudaError_t scan_launch(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
+cudaError_t scan_launch(const mmfree_cuda_ssm_args& a, int sms, cudaStream_t s) {
   constexpr size_t kSmem = sizeof(typename S::Shared);
   const int blocks = static_cast<int>(ceil_div(static_cast<int64_t>(a.channels / a.groups), S::kChannels));
+  // Few CTAs and long sequences: clusters of 8 or 4 split each sequence, as many as two CTAs an SM hold. One sequence of
+  // 8192 tokens x 1024 channels (bf16, 32 CTAs): 334 us in one piece, 145 us in 8; 2048 x 2048 (64 CTAs): 86.5 us in one
+  // piece, 74.8 us in 4.
+  const int64_t ctas = static_cast<int64_t>(blocks) * static_cast<int64_t>(a.groups * a.seqs);
+  const bool long_ones = a.tokens / a.seqs >= 512;
+  const int splits = !S::kMaySplit || !long_ones ? 1 : ctas * 4 <= sms ? 8 : ctas * 2 <= sms ? 4 : 1;
   // channel blocks fastest: consecutive CTAs go to different SMs, so every SM gets its share of each sequence
-  const dim3 grid(static_cast<unsigned>(blocks * a.groups), static_cast<unsigned>(a.seqs));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks * a.groups * splits), static_cast<unsigned>(a.seqs));
+  cfg.blockDim = dim3(S::kScan + S::kHelpers);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = static_cast<unsigned>(splits);
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
   if (kSmem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(scan_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
     if (e != cudaSuccess) return e;
   }
-  return launch_k(scan_kernel<S>, grid, dim3(S::kScan + S::kHelpers), kSmem, s, false, a, blocks);
+  return cudaLaunchKernelEx(&cfg, scan_kernel<S>, a, blocks, splits);
 }
 
 template <typename T, int kBytes>
 cudaError_t scan_states(const mmfree_cuda_ssm_args& a, int sms, cudaStream_t s) {
-  if (a.states <= 4) return scan_launch<ScanShape<T, 1, 4, 1, 8, 128, 128, 2, kBytes>>(a, s);
-  if (a.states <= 8) return scan_launch<ScanShape<T, 2, 4, 1, 16, 128, 128, 2, kBytes>>(a, s);
+  if (a.states <= 4) return scan_launch<ScanShape<T, 1, 4, 1, 8, 128, 128, 2, kBytes>>(a, sms, s);
+  if (a.states <= 8) return scan_launch<ScanShape<T, 2, 4, 1, 16, 128, 128, 2, kBytes>>(a, sms, s);
   if (a.states <= 16) {
     // Two channels a lane (half the reads of B and C) where CTAs of 32 channels are several an SM, else one, on
     // twice the warps: 16384 tokens in 8 sequences x 5120 channels take 658 against 668 us, one sequence of 4099
     // x 4096 (one CTA an SM) 260 against 162 us.
     if (static_cast<int64_t>(a.channels * a.seqs) >= 32 * 3 * static_cast<int64_t>(sms))
-      return scan_launch<ScanShape<T, 4, 4, 2, 16, 64, 64, 4, kBytes>>(a, s);
-    return scan_launch<ScanShape<T, 4, 4, 1, 32, 128, 128, 2, kBytes>>(a, s);
+      return scan_launch<ScanShape<T, 4, 4, 2, 16, 64, 64, 4, kBytes>>(a, sms, s);
+    return scan_launch<ScanShape<T, 4, 4, 1, 32, 128, 128, 2, kBytes>>(a, sms, s);
   }
-  if (a.states <= 32) return scan_launch<ScanShape<T, 8, 4, 1, 32, 128, 128, 2, kBytes>>(a, s);
-  if (a.states <= 64) return scan_launch<ScanShape<T, 16, 4, 1, 32, 128, 128, 2, kBytes>>(a, s);
-  if (a.states <= 128) return scan_launch<ScanShape<T, 32, 4, 2, 16, 128, 128, 2, kBytes>>(a, s);
-  return scan_launch<ScanShape<T, 32, 8, 1, 8, 128, 128, 2, kBytes>>(a, s);
+  if (a.states <= 32) return scan_launch<ScanShape<T, 8, 4, 1, 32, 128, 128, 2, kBytes>>(a, sms, s);
+  if (a.states <= 64) return scan_launch<ScanShape<T, 16, 4, 1, 32, 128, 128, 2, kBytes>>(a, sms, s);
+  if (a.states <= 128) return scan_launch<ScanShape<T, 32, 4, 2, 16, 128, 128, 2, kBytes>>(a, sms, s);
+  return scan_launch<ScanShape<T, 32, 8, 1, 8, 128, 128, 2, kBytes>>(a, sms, s);
 }
 
 template <typename T>

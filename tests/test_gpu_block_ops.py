@@ -315,7 +315,9 @@ def test_selective_scan(cuda, channels, states, groups, extra, kind):
 
 
 @pytest.mark.parametrize("kind", ["fp32", "bf16"])
-@pytest.mark.parametrize("lens,channels,states", [([3000], 8, 16), ([700, 1, 0, 1300], 40, 16), ([1500], 4, 128), ([520], 130, 3)])
+@pytest.mark.parametrize("lens,channels,states", [
+    ([3000], 8, 16), ([700, 1, 0, 1300], 40, 16), ([1500], 4, 128), ([520], 130, 3), ([4000, 0, 2, 900, 3000], 64, 16),
+    ([2500], 33, 16), ([1100], 12, 200), ([1300, 700], 72, 7)])
 def test_selective_scan_long(cuda, lens, channels, states, kind):
     starts = R.starts_of(lens)
     p = ssm_inputs(starts[-1], channels, states, 1, kind, 7, len(lens))
