@@ -8,9 +8,12 @@
 // issue slots allow at the memory's rate, so the products run on the tensor cores (the warp
 // instruction m16n8k16: 16 weight rows x 8 activation rows x 16 columns; tcgen05 would need the
 // unpacked weights in shared or tensor memory first, an extra trip for operands used once).
-// u - z is a small whole number, exact in fp16 and bf16; int8 and e4m3 rows are exact in fp16;
-// fp32 rows are cut into three bf16 parts of 8 bits each, exactly. The products are therefore
-// exact, summed in fp32, and a group's sum is scaled once.
+// u - z is a small whole number, exact in fp16 and bf16; e4m3 rows are exact in fp16; fp32 rows
+// are cut into three bf16 parts of 8 bits each, exactly. The products are therefore exact, summed
+// in fp32, and a group's sum is scaled once. For int8 rows the codes stay whole numbers:
+// m16n8k32 of u8 codes and s8 rows, summed in 32 bits, and a group's sum of (u - z) x is the sum
+// of u x minus z times the sum of x, which an operand of ones gives (2048 -> 32000: I8_BEFORE us as
+// fp16, I8_AFTER us).
 //
 // The order of a product's columns is free as long as weights and activations agree, so a lane
 // takes 8 consecutive columns of its weight row, one word of the row-major codes: no repacked
@@ -117,14 +120,6 @@ __device__ __forceinline__ void split_x(const uint32_t (&w)[RowType<kType>::kWor
     b[0][1] = __byte_perm(w[0], w[2], 0x7632);
     b[0][2] = __byte_perm(w[1], w[3], 0x5410);
     b[0][3] = __byte_perm(w[1], w[3], 0x7632);
-  } else if constexpr (kType == MMFREE_T_S8) {
-    const uint32_t lo = w[0] ^ 0x80808080u, hi = w[1] ^ 0x80808080u;  // x + 128 in 0..255
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // 0x64nn is 1024 + nn in fp16
-      const uint32_t v = (__byte_perm(lo, hi, i | ((4 + i) << 8)) & 0x00FF00FFu) | 0x64006400u;
-      b[0][i] = h2_sub(v, 0x64806480u);
-    }
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -158,6 +153,11 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
   else
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_u8s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // 16 bytes of which the first `bytes` are read and the others become 0.
@@ -301,6 +301,8 @@ __global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCta
       for (int group = 0; r < runs; ++group) {
         const int stop = min(runs, ((g0 + group + 1) * a.group - k0) / 32);
         float part[kBlocks][kTiles][4] = {};
+        constexpr bool kWhole = kType == MMFREE_T_S8;
+        int whole_part[kBlocks][kTiles][4] = {}, xsum[kTiles][4] = {};  // kWhole
         uint32_t zero[kBlocks][2], zero16[kBlocks][2];
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)
@@ -309,7 +311,31 @@ __global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCta
             zero[b][h] = mine.zero[group][16 * b + 8 * h + g];
             zero16[b][h] = X::kBf16 ? 0 : h2_sub(0x63806380u, zero[b][h]);  // 960 - (1024 + z)
           }
+        const auto word = [&](int b, int h) {
+          const int row = 16 * b + 8 * h + g;
+          if constexpr (kAligned) return words[row * kChunks * 4 + (((r ^ g) & 7) * 4 + t)];
+          const int at = row * kChunks * 4 + r * 4 + t + (offset[b][h] >> 2);
+          return __funnelshift_r(words[at], words[min(at + 1, kRows * kChunks * 4 - 1)], 8 * (offset[b][h] & 3));
+        };
         const auto run = [&](const uint32_t (&xw)[kTiles][X::kWords]) {
+          if constexpr (kWhole) {
+            // a word's codes 0, 2, 4, 6 and 1, 3, 5, 7 as bytes, and the row's columns in that order
+            uint32_t x0[kTiles], x1[kTiles];
+#pragma unroll
+            for (int c = 0; c < kTiles; ++c) {
+              x0[c] = __byte_perm(xw[c][0], xw[c][1], 0x6420);
+              x1[c] = __byte_perm(xw[c][0], xw[c][1], 0x7531);
+              mma_u8s8(xsum[c], 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, x0[c], x1[c]);
+            }
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+              const uint32_t u0 = word(b, 0), u1 = word(b, 1), even = 0x0F0F0F0Fu;
+#pragma unroll
+              for (int c = 0; c < kTiles; ++c)
+                mma_u8s8(whole_part[b][c], u0 & even, u1 & even, (u0 >> 4) & even, (u1 >> 4) & even, x0[c], x1[c]);
+            }
+            return;
+          }
           uint32_t xb[kTiles][X::kParts][4];
 #pragma unroll
           for (int c = 0; c < kTiles; ++c) split_x<kType>(xw[c], xb[c]);
@@ -317,17 +343,7 @@ __global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCta
           for (int b = 0; b < kBlocks; ++b) {
             uint32_t p[2][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int row = 16 * b + 8 * h + g;
-              uint32_t u;
-              if constexpr (kAligned) {
-                u = words[row * kChunks * 4 + (((r ^ g) & 7) * 4 + t)];
-              } else {
-                const int at = row * kChunks * 4 + r * 4 + t + (offset[b][h] >> 2);
-                u = __funnelshift_r(words[at], words[min(at + 1, kRows * kChunks * 4 - 1)], 8 * (offset[b][h] & 3));
-              }
-              split_codes<X::kBf16>(u, zero[b][h], zero16[b][h], p[h]);
-            }
+            for (int h = 0; h < 2; ++h) split_codes<X::kBf16>(word(b, h), zero[b][h], zero16[b][h], p[h]);
 #pragma unroll
             for (int c = 0; c < kTiles; ++c)
 #pragma unroll
@@ -373,7 +389,11 @@ __global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCta
           for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
+            {
+              if constexpr (kWhole)  // the zero point is the low byte of 1024 + z
+                part[b][c][j] = static_cast<float>(whole_part[b][c][j] - static_cast<int>(zero[b][j >> 1] & 0xFFu) * xsum[c][j & 1]);
               total[b][c][j] = fmaf(mine.scale[group][16 * b + 8 * (j >> 1) + g], part[b][c][j] * xs[j & 1], total[b][c][j]);
+            }
         }
       }
     }
