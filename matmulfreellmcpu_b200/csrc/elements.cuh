@@ -71,6 +71,25 @@ __device__ __forceinline__ void store_row(T* p, int n, const float (&r)[V]) {
   }
 }
 
+// Two values rounded to T: as they lie in memory, and as fp32 again.
+__device__ __forceinline__ uint32_t round2(float& lo, float& hi, __nv_bfloat16) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  uint32_t w;
+  memcpy(&w, &p, 4);
+  lo = __uint_as_float(w << 16);
+  hi = __uint_as_float(w & 0xFFFF0000u);
+  return w;
+}
+__device__ __forceinline__ uint32_t round2(float& lo, float& hi, __half) {
+  const __half2 p = __floats2half2_rn(lo, hi);
+  uint32_t w;
+  memcpy(&w, &p, 4);
+  const float2 f = __half22float2(p);
+  lo = f.x;
+  hi = f.y;
+  return w;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 constexpr float kLog2E = 1.44269504088896341f;

@@ -12,14 +12,15 @@
 // are cut into three bf16 parts of 8 bits each, exactly. The products are therefore exact, summed
 // in fp32, and a group's sum is scaled once. For int8 rows the codes stay whole numbers:
 // m16n8k32 of u8 codes and s8 rows, summed in 32 bits, and a group's sum of (u - z) x is the sum
-// of u x minus z times the sum of x, which an operand of ones gives (2048 -> 32000: I8_BEFORE us as
-// fp16, I8_AFTER us).
+// of u x minus z times the sum of x, which an operand of ones gives (one row, 2048 -> 32000: 19.1 us as
+// fp16, 14.5 us).
 //
 // The order of a product's columns is free as long as weights and activations agree, so a lane
 // takes 8 consecutive columns of its weight row, one word of the row-major codes: no repacked
 // copy of the weights. The words come through shared memory, filled by asynchronous copies two
 // turns ahead; rolled loops over it keep the code small (with the words in registers the
-// unrolled loops were bound by instruction fetches: 22 instead of KERNEL_US us for 2048 -> 32000).
+// unrolled loops were bound by instruction fetches: 20.4 instead of 15.2 us for 16 fp32 rows,
+// 5632 -> 2048).
 #include "block_ops.h"
 #include "common.cuh"
 #include "elements.cuh"

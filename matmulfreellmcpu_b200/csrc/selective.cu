@@ -76,6 +76,8 @@ __device__ __forceinline__ void conv_token(const float (*in)[V], const float (&w
     for (int i = 0; i < V; ++i) y[i] = silu_f32(y[i]);
 }
 
+// Bound by the bytes in fp32 (16384 x 5120 x 4 taps: 113 us, 6.0 TB/s), by the issue slots and the sigmoid's special
+// functions in 16 bits (68 us, 4.9 TB/s). A thread keeps its channels' last inputs in registers.
 // A CTA owns a tile of `rows` tokens for a block of channels. The tile in which a sequence
 // begins reads that sequence's old state, writes the new one, and computes every token whose
 // window still reaches into the old state, even those behind the tile's end, which the tiles
@@ -220,7 +222,8 @@ cudaError_t conv_launch(const mmfree_cuda_conv_args& a, bool step, cudaStream_t 
   const unsigned blocks = static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.channels), 128 * V));
   mark_device();
   if (step) return launch_k(conv_step_kernel<T, W, V>, dim3(blocks, static_cast<unsigned>(a.seqs)), dim3(128), 0, s, false, a);
-  // tokens of a tile: 64, of which W - 1 are read twice, fewer where the tiles would not fill the SMs (a small call)
+  // Tokens of a tile: 64, before which W - 1 are read once more (16384 x 5120 bf16: 68 us; 76 us with tiles of 128),
+  // fewer where the tiles would not fill the 148 SMs (300 x 2048: 8.0 us, 14.6 us with 64).
   int rows = 64;
   while (rows > 8 && static_cast<int64_t>(blocks) * ceil_div(static_cast<int64_t>(a.tokens), rows) < 4 * 148) rows /= 2;
   while (ceil_div(static_cast<int64_t>(a.tokens), rows) > 65535) rows *= 2;  // grid.y is 16 bits
@@ -244,9 +247,10 @@ cudaError_t conv_width(const mmfree_cuda_conv_args& a, bool step, cudaStream_t s
 
 template <typename T>
 cudaError_t conv_type(const mmfree_cuda_conv_args& a, bool step, cudaStream_t s) {
-  constexpr int V = 16 / sizeof(T);  // channels of a 16-byte access
-  const bool vec = a.channels % V == 0 && a.ldx % V == 0 && a.ld_out % V == 0 && aligned16(a.x) && aligned16(a.out) &&
-                   aligned16(a.state) && aligned16(a.weight);
+  constexpr int V = 4;  // channels of a thread (with 8 of a 16-bit type, half as many warps: 76 instead of 68 us)
+  const auto fits = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % (V * sizeof(T)) == 0; };
+  const bool vec = a.channels % V == 0 && a.ldx % V == 0 && a.ld_out % V == 0 && fits(a.x) && fits(a.out) && fits(a.state) &&
+                   aligned16(a.weight);
   return vec ? conv_width<T, V>(a, step, s) : conv_width<T, 1>(a, step, s);
 }
 
@@ -278,8 +282,8 @@ __device__ __forceinline__ float softplus_f32(float v) {
 }
 
 // One token of each of kStreams streams: `lanes` lanes (a power of two) a channel, kStates neighbouring states a lane,
-// kVec: read and written by 16 bytes. Bound by the state's bytes, which have to be in flight together: four streams a
-// thread where there are enough. Every lane repeats its channel's softplus and gate, which costs less than passing
+// kVec: read and written by 16 bytes. Bound by the state's bytes (256 streams: 3.2 TB/s), which have to be in flight
+// together: four streams a thread where there are enough. Every lane repeats its channel's softplus and gate, which costs less than passing
 // them on.
 template <typename T, int kStates, int kStreams, bool kVec>
 __global__ void __launch_bounds__(256) step_kernel(mmfree_cuda_ssm_args a, int lanes) {
@@ -410,7 +414,7 @@ struct ScanShape {
   static constexpr int kCtas = kCtas_;                          // CTAs an SM that the registers leave room for
   static constexpr int kBytes = kBytes_;                        // of an access: 16 or 4, copied asynchronously, or 0: one element
   static constexpr bool kVec = kBytes > 0;
-  static constexpr bool kMaySplit = kCtas < 4;                  // the shape for many CTAs is never short of them
+  static constexpr bool kMaySplit = kCtas < 4;                  // the shape for short sequences never splits them
   static constexpr int kN = kLanes * kStates;                   // states, padded
   static constexpr int kChannels = kScan / kLanes * kPer;
   static constexpr int kWide = kVec ? kBytes / sizeof(T) : 1;
@@ -442,6 +446,10 @@ struct ScanShape {
 // 0, plus the state before it times exp(A * the sum of the piece's deltas): so the pieces between the first and the last
 // run without outputs first, then every piece but the first starts from the states and sums of those before it, read
 // from their shared memory. Two passes for a sequence, each over 1 / splits of it.
+// Bound by the exponentials, one for each token, channel and state: 16 a clock and SM, 385 us with the helpers' for
+// 16384 tokens x 5120 channels x 16 states, where the kernel takes 646 us; the special-function unit is busy 60% of the
+// time, the rest goes to the two halves' waits for each other and for its latency. An eighth or a quarter of the
+// exponentials as polynomials on the multiply-add pipe changed nothing (663 and 693 against 657 us), nor did more CTAs an SM.
 // What a turn of the recurrence reads from shared memory bounds it next to the special-function unit (128 bytes of
 // registers a clock): kPer channels a lane share one read of B and C.
 template <typename S>
@@ -822,10 +830,11 @@ cudaError_t scan_states(const mmfree_cuda_ssm_args& a, int sms, cudaStream_t s) 
   if (a.states <= 4) return scan_launch<ScanShape<T, 1, 4, 1, 8, 128, 128, 2, kBytes>>(a, sms, s);
   if (a.states <= 8) return scan_launch<ScanShape<T, 2, 4, 1, 16, 128, 128, 2, kBytes>>(a, sms, s);
   if (a.states <= 16) {
-    // Two channels a lane (half the reads of B and C) where CTAs of 32 channels are several an SM, else one, on
-    // twice the warps: 16384 tokens in 8 sequences x 5120 channels take 658 against 668 us, one sequence of 4099
-    // x 4096 (one CTA an SM) 260 against 162 us.
-    if (static_cast<int64_t>(a.channels * a.seqs) >= 32 * 3 * static_cast<int64_t>(sms))
+    // Short sequences on many CTAs: two channels a lane (half the reads of B and C) and tiles of 16 tokens, which leave
+    // less behind a sequence's end: 300 tokens in 16 sequences x 2048 channels (fp32) take 14.3 against 16.7 us. Long
+    // ones the other way: 16384 tokens in 8 sequences x 5120 channels (bf16) 646 against 657 us, one sequence of
+    // 4099 x 4096 160 against 203 us.
+    if (static_cast<int64_t>(a.channels * a.seqs) >= 32 * 3 * static_cast<int64_t>(sms) && a.tokens / a.seqs < 512)
       return scan_launch<ScanShape<T, 4, 4, 2, 16, 64, 64, 4, kBytes>>(a, sms, s);
     return scan_launch<ScanShape<T, 4, 4, 1, 32, 128, 128, 2, kBytes>>(a, sms, s);
   }
@@ -851,7 +860,8 @@ cudaError_t scan_type(const mmfree_cuda_ssm_args& a, int sms, cudaStream_t s) {
 template <typename T, int kStates, bool kVec>
 cudaError_t step_launch(const mmfree_cuda_ssm_args& a, int lanes, cudaStream_t s) {
   const unsigned blocks = static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.channels) * lanes, 256));
-  // four streams a thread where one stream a thread would be more threads than the SMs hold at once
+  // four streams a thread where one stream a thread would be more threads than the 148 SMs hold at once (4096 x 16
+  // states: 64 streams 13.4 against 15.9 us, 256 streams 45.3 against 57.5 us)
   if (static_cast<int64_t>(blocks) * static_cast<int64_t>(a.seqs) > 148 * 8)
     return launch_k(step_kernel<T, kStates, 4, kVec>, dim3(blocks, static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.seqs), 4))), dim3(256), 0, s, false, a, lanes);
   return launch_k(step_kernel<T, kStates, 1, kVec>, dim3(blocks, static_cast<unsigned>(a.seqs)), dim3(256), 0, s, false, a, lanes);
