@@ -282,8 +282,8 @@ __device__ __forceinline__ float softplus_f32(float v) {
 }
 
 // One token of each of kStreams streams: `lanes` lanes (a power of two) a channel, kStates neighbouring states a lane,
-// kVec: read and written by 16 bytes. Bound by the state's bytes (256 streams: 3.2 TB/s), which have to be in flight
-// together: four streams a thread where there are enough. Every lane repeats its channel's softplus and gate, which costs less than passing
+// kVec: read and written by 16 bytes. Bound by its issue slots (67% busy at 256 streams, 3.2 TB/s) and by how many of
+// the state's bytes are in flight together: four streams a thread where there are enough. Every lane repeats its channel's softplus and gate, which costs less than passing
 // them on.
 template <typename T, int kStates, int kStreams, bool kVec>
 __global__ void __launch_bounds__(256) step_kernel(mmfree_cuda_ssm_args a, int lanes) {
