@@ -294,7 +294,9 @@ __global__ void __launch_bounds__(256) step_kernel(mmfree_cuda_ssm_args a, int l
   const int64_t dd = live ? d : channels - 1;
   const int n = lane * kStates, left = states - n;
   const int64_t group = dd / (channels / static_cast<int64_t>(a.groups));
-  // all streams' loads without a branch or a use between them: an absent stream reads another one's
+  // all streams' loads without a branch or a use between them. One behind the last stream reads that one's; a stream that
+  // is not there (a negative or bad slot) reads its channel's row of A in place of a state, since no state is its own and
+  // the pool may hold none.
   bool there[kStreams];
   float* state[kStreams];
   float h[kStreams][kStates], rate[kStates] = {};
@@ -304,7 +306,7 @@ __global__ void __launch_bounds__(256) step_kernel(mmfree_cuda_ssm_args a, int l
   for (int k = 0; k < kStreams; ++k) {
     const int64_t seq = min(seq0 + k, seqs - 1), slot = sequence_slot(a.slots, static_cast<int64_t>(a.slot_count), seq);
     there[k] = slot >= 0 && seq0 + k < seqs;
-    state[k] = a.state + (max(slot, int64_t(0)) * channels + dd) * states + min(n, states - 1);
+    state[k] = (slot < 0 ? const_cast<float*>(a.A) : a.state + slot * channels * states) + dd * states + min(n, states - 1);
   }
 #pragma unroll
   for (int k = 0; k < kStreams; ++k) {

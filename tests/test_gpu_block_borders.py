@@ -1,0 +1,69 @@
+"""GPU tests of the recurrent-block operators at the borders of their ranges: infinities, extreme rows, sequences that break
+the rules, padded pools, and what torch records about tensors that are written in place."""
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+import torch
+
+import block_ref as R
+from matmulfreellmcpu_b200 import _lib, api
+from test_gpu_block_ops import SENTINEL, rng, ssm_inputs
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("streams,channels,states", [(3, 32, 16), (5, 33, 5), (77, 1200, 16)])
+def test_a_batch_of_padding_over_an_empty_pool(cuda, streams, channels, states):
+    """The C ABI's step with no state in the pool and no stream that is there: nothing is read from the pool, nothing is
+    written, and only a slot that is not negative is reported."""
+    d = {k: v.to(cuda) for k, v in ssm_inputs(streams, channels, states, 1, "fp32", 3, 1).items()}
+    w, conv = torch.randn(channels, 4, device=cuda), torch.zeros(1, 3, channels, device=cuda)
+    slots = torch.full((streams,), -1, dtype=torch.int32, device=cuda)
+    out, state = torch.full((streams, channels), SENTINEL, device=cuda), d["state"].clone()
+    torch.cuda.synchronize()
+    s = _lib.SsmArgs(out=out.data_ptr(), x=d["x"].data_ptr(), dt=d["dt"].data_ptr(), z=d["z"].data_ptr(), B=d["B"].data_ptr(),
+                     C=d["C"].data_ptr(), A=d["A"].data_ptr(), state=state.data_ptr(), slots=slots.data_ptr(), ld_out=channels,
+                     ldx=channels, ld_dt=channels, ldz=channels, ldb=states, ldc=states, tokens=streams, seqs=streams, slot_count=0,
+                     channels=channels, states=states, groups=1, type=_lib.T_F32, dt_softplus=1)
+    c = _lib.ConvArgs(out=out.data_ptr(), x=d["x"].data_ptr(), weight=w.data_ptr(), state=conv.data_ptr(), slots=slots.data_ptr(),
+                      ld_out=channels, ldx=channels, tokens=streams, seqs=streams, slot_count=0, channels=channels, width=4,
+                      type=_lib.T_F32, silu=1)
+    stream = torch.cuda.current_stream().cuda_stream
+    api.kernel_status()
+    for bad in (False, True):
+        if bad:
+            slots[streams // 2] = 0
+        for call, args in ((_lib.lib().mmfree_cuda_selective_step, s), (_lib.lib().mmfree_cuda_causal_conv_step, c)):
+            _lib.check(call(C.byref(args), stream))
+            if bad:
+                with pytest.raises(api.MmfreeError) as e:
+                    api.kernel_status()
+                assert e.value.code == _lib.E_RANGE
+            else:
+                api.kernel_status()
+    assert (out == SENTINEL).all() and torch.equal(state, d["state"]) and (conv == 0).all()
+
+
+@pytest.mark.parametrize("channels,states", [(1200, 16), (1200, 5), (600, 40)])
+def test_padded_streams_among_four_of_a_thread(cuda, channels, states):
+    """Streams that are not there, alone, several together and last, where a thread has four streams; the pool's states that no
+    stream has are NaN."""
+    streams = 77
+    pool = streams + 3
+    p = ssm_inputs(streams, channels, states, 1, "bf16", channels, pool)
+    slots = torch.randperm(pool, generator=rng(2))[:streams].to(torch.int32)
+    slots[torch.tensor([1, 8, 9, 10, 11, 40, 42, 76])] = -1
+    idle = [i for i in range(pool) if i not in slots.tolist()]
+    p["state"][idle] = torch.nan
+    want, bound, new, nbound = R.ssm_ref(p["x"], p["dt"], p["A"], p["B"], p["C"], p["D"], p["z"], p["dt_bias"], True, p["state"],
+                                         list(range(streams + 1)), slots)
+    d = {k: v.to(cuda) for k, v in p.items()}
+    out = torch.full_like(d["x"], SENTINEL)
+    api.selective_step(d["x"], d["dt"], d["A"], d["B"], d["C"], d["state"], d["D"], d["z"], d["dt_bias"], slots=slots.to(cuda), out=out)
+    inside, live = ~torch.isnan(want), [i for i in range(pool) if i not in idle]
+    assert ((out.cpu().double() - want).abs()[inside] <= bound[inside]).all() and (out.cpu()[~inside] == SENTINEL).all()
+    state = d["state"].cpu()
+    assert ((state.double() - new).abs()[live] <= nbound[live]).all() and torch.isnan(state[idle]).all()
+    api.kernel_status()
