@@ -426,6 +426,11 @@ struct ScanShape {
   static constexpr int kOwn = (kTile + kRows - 1) / kRows;      // tokens of a helper
   static constexpr int kBC = (kTile * kN / VB + kHelpers - 1) / kHelpers;  // vectors of B (and of C) of a helper
   static constexpr int kStages = kVec ? 4 : 1;
+  // Places behind the last state hold copies of the first ones, each with its share of C (shares of a half or a quarter,
+  // which are exact): with zeros there, an infinite x would bring 0 * infinity into the sum. kN is the power of two next to
+  // the number of states (or 4), so that a state has one copy at most, and the only one of a single state has three.
+  __device__ static int source(int n, int states, int width) { return n < states ? n : min(n - states, states - width); }
+  __device__ static float share(int n, int states) { return states == 1 ? 0.25f : n < kN - states || n >= states ? 0.5f : 1.0f; }
   struct Raw {  // one tile as it lies in memory; every helper reads what it copied itself
     Pack<T, V> x[kOwn][kHelpers], dt[kOwn][kHelpers], z[kOwn][kHelpers];
     Pack<T, VB> b[kBC][kHelpers], c[kBC][kHelpers];
@@ -504,9 +509,9 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
         float hv[2], rv[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int n = lane * kStates + 2 * j + i;
-          hv[i] = n < states && pool && mine_first ? pool[d * states + n] : 0.0f;
-          rv[i] = n < states ? a.A[d * states + n] * kLog2E : 0.0f;
+          const int n = S::source(lane * kStates + 2 * j + i, states, 1);
+          hv[i] = pool && mine_first ? pool[d * states + n] : 0.0f;
+          rv[i] = a.A[d * states + n] * kLog2E;
         }
         h[c][j] = pack2(hv[0], hv[1]);
         rate[c][j] = pack2(rv[0], rv[1]);
@@ -679,7 +684,7 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
       }
 #pragma unroll
       for (int i = 0; i < kBC; ++i) {
-        const int at = (tid + i * kHelpers) * VB, n = min(at % kN, states - VB);
+        const int at = (tid + i * kHelpers) * VB, n = S::source(at % kN, states, VB);
         if (kTile * kN / VB % kHelpers && at >= kTile * kN) break;
         const int64_t t = t0 + min(at / kN, most);
         fetch(&raw.b[i][tid], pb + t * ldb + n);
@@ -737,8 +742,8 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
       Pack<float, VB> vb, vc;
 #pragma unroll
       for (int v = 0; v < VB; ++v) {
-        vb.v[v] = n < states && at / kN < left ? to_f32(rb.v[v]) : 0.0f;  // 0 behind the end too: 0 * inf is not 0
-        vc.v[v] = n < states ? to_f32(rc.v[v]) : 0.0f;
+        vb.v[v] = at / kN < left ? to_f32(rb.v[v]) : 0.0f;  // 0 behind the end too: 0 * inf is not 0
+        vc.v[v] = to_f32(rc.v[v]) * S::share(n + v, states);
       }
       *reinterpret_cast<Pack<float, VB>*>(&sh.b[buf][at / kN][n]) = vb;
       *reinterpret_cast<Pack<float, VB>*>(&sh.c[buf][at / kN][n]) = vc;

@@ -9,7 +9,7 @@ import torch
 
 import block_ref as R
 from matmulfreellmcpu_b200 import _lib, api
-from test_gpu_block_ops import SENTINEL, rng, ssm_inputs
+from test_gpu_block_ops import SENTINEL, close, rng, run_ssm, ssm_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,37 @@ def test_padded_streams_among_four_of_a_thread(cuda, channels, states):
     state = d["state"].cpu()
     assert ((state.double() - new).abs()[live] <= nbound[live]).all() and torch.isnan(state[idle]).all()
     api.kernel_status()
+
+
+def same_values(got, want, bound, what):
+    """Infinities and NaN where the reference has them, the finite values within the bound."""
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{what}: NaN"
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf], want[inf]), f"{what}: infinities"
+    finite = torch.isfinite(want)
+    close(got[finite], want[finite], bound[finite], what)
+
+
+def ssm_reference(p, starts, slots=None, **kw):
+    return R.ssm_ref(p["x"], p["dt"], p["A"], p["B"], p["C"], p["D"], p["z"], p["dt_bias"], True, p["state"], starts, slots, **kw)
+
+
+@pytest.mark.parametrize("states", [1, 2, 3, 5, 7, 12, 20, 100, 129])
+@pytest.mark.parametrize("channels", [24, 23])
+def test_an_infinite_input_with_padded_states(cuda, channels, states):
+    """An infinity in x makes the states of its channel infinite and leaves the others alone, whatever the shape's number of
+    states is; a prompt and its tokens one by one give the same."""
+    p = ssm_inputs(20, channels, states, 1, "fp32", states, 1)
+    p["B"], p["C"] = p["B"].abs() + 0.1, p["C"].abs() + 0.1
+    p["x"][6, 5] = torch.inf
+    p["D"] = p["D"].abs() + 0.1
+    want, bound, new, nbound = ssm_reference(p, [0, 20])
+    out, state = run_ssm(cuda, p, [0, 20], None, 0)
+    same_values(out, want, bound, "prompt")
+    same_values(state, new, nbound, "state")
+    d = {k: v.to(cuda) for k, v in p.items()}
+    for t in range(20):
+        row = slice(t, t + 1)
+        y = api.selective_step(d["x"][row], d["dt"][row], d["A"], d["B"][row], d["C"][row], d["state"], d["D"], d["z"][row], d["dt_bias"])
+        same_values(y, want[row], bound[row], f"token {t}")
