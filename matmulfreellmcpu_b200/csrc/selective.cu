@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(256) step_kernel(mmfree_cuda_ssm_args a, int l
     for (int o = lanes >> 1; o; o >>= 1) y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
     if (!live || !there[k]) continue;
     if (left > 0) store_row<kVec>(state[k], left, h[k]);
-    y = fmaf(skip, xk, y);
+    if (a.D) y = fmaf(skip, xk, y);  // without D not 0 * x, which may be 0 * infinity
     if (a.z) y *= silu_f32(z[k][0]);
     if (lane == 0) static_cast<T*>(a.out)[(seq0 + k) * static_cast<int64_t>(a.ld_out) + dd] = from_f32<T>(y);
   }
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
     skip[v] = a.D ? a.D[d + v] : 0.0f;
     bias[v] = a.dt_bias ? a.dt_bias[d + v] : 0.0f;
   }
-  const bool gate = a.z != nullptr, softplus = a.dt_softplus != 0;
+  const bool gate = a.z != nullptr, skips = a.D != nullptr, softplus = a.dt_softplus != 0;
   const int64_t ldx = static_cast<int64_t>(a.ldx), ldt = static_cast<int64_t>(a.ld_dt), ldz = static_cast<int64_t>(a.ldz),
                 ldb = static_cast<int64_t>(a.ldb), ldc = static_cast<int64_t>(a.ldc), ldo = static_cast<int64_t>(a.ld_out);
   const T* px = static_cast<const T*>(a.x) + b * ldx + d;
@@ -767,7 +767,10 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
       const Pack<float, V> p = *reinterpret_cast<const Pack<float, V>*>(&sh.y[buf][t][ch]);
       float y[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) y[v] = fmaf(skip[v], to_f32(rx.v[v]), p.v[v]);
+      for (int v = 0; v < V; ++v) y[v] = p.v[v];
+      if (skips)  // without D not 0 * x, which may be 0 * infinity
+#pragma unroll
+        for (int v = 0; v < V; ++v) y[v] = fmaf(skip[v], to_f32(rx.v[v]), y[v]);
       if (gate)
 #pragma unroll
         for (int v = 0; v < V; ++v) y[v] *= silu_f32(to_f32(rz.v[v]));

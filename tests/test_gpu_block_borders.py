@@ -101,3 +101,19 @@ def test_an_infinite_input_with_padded_states(cuda, channels, states):
         row = slice(t, t + 1)
         y = api.selective_step(d["x"][row], d["dt"][row], d["A"], d["B"][row], d["C"][row], d["state"], d["D"], d["z"][row], d["dt_bias"])
         same_values(y, want[row], bound[row], f"token {t}")
+
+
+def test_an_infinite_input_without_a_skip(cuda):
+    """Without D nothing of x is added to what the states give: no 0 * infinity."""
+    p = ssm_inputs(20, 24, 16, 1, "fp32", 4, 1)
+    p["B"], p["C"], p["D"] = p["B"].abs() + 0.1, p["C"].abs() + 0.1, None
+    p["x"][6, 5] = torch.inf
+    want, bound, _, _ = ssm_reference(p, [0, 20])
+    assert torch.isinf(want[6:, 5]).all()
+    out, _ = run_ssm(cuda, p, [0, 20], None, 0, drop=("D",))
+    same_values(out, want, bound, "prompt")
+    d = {k: None if v is None else v.to(cuda) for k, v in p.items()}
+    for t in range(8):
+        row = slice(t, t + 1)
+        y = api.selective_step(d["x"][row], d["dt"][row], d["A"], d["B"][row], d["C"][row], d["state"], None, d["z"][row], d["dt_bias"])
+        same_values(y, want[row], bound[row], f"token {t}")
