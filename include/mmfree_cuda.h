@@ -252,7 +252,7 @@ typedef struct {
   const void* z;         /* [tokens, channels] (nullable: no gate) */
   const void* B;         /* [tokens, groups, states]: channel d uses group d / (channels / groups) */
   const void* C;         /* [tokens, groups, states] */
-  const float* A;        /* [channels, states] */
+  const float* A;        /* [channels, states]; an infinity counts as the largest finite number */
   const float* D;        /* [channels] (nullable) */
   const float* dt_bias;  /* [channels] (nullable) */
   float* state;          /* [slot_count, channels, states]; updated (nullable in a scan: zeros,

@@ -281,6 +281,10 @@ __device__ __forceinline__ float softplus_f32(float v) {
   return fmaf(2.0f, l, fmaxf(v, 0.0f));
 }
 
+// A rate that is infinite (A itself, or its product with log2(e)) counts as the largest finite one: a decay of 0 after any
+// step above 1e-36, as its own would be, and of 1, not NaN, where delta is 0, as behind a sequence's end.
+__device__ __forceinline__ float finite_rate(float v) { return isinf(v) ? copysignf(3.402823466e38f, v) : v; }
+
 // One token of each of kStreams streams: `lanes` lanes (a power of two) a channel, kStates neighbouring states a lane,
 // kVec: read and written by 16 bytes. Bound by its issue slots (67% busy at 256 streams, 3.2 TB/s) and by how many of
 // the state's bytes are in flight together: four streams a thread where there are enough. Every lane repeats its channel's softplus and gate, which costs less than passing
@@ -332,6 +336,8 @@ __global__ void __launch_bounds__(256) step_kernel(mmfree_cuda_ssm_args a, int l
     if (a.z) z[k].load(static_cast<const T*>(a.z) + seq * static_cast<int64_t>(a.ldz) + dd);
   }
   if (left > 0) load_row<kVec>(a.A + dd * states + n, left, rate);
+#pragma unroll
+  for (int i = 0; i < kStates; ++i) rate[i] = finite_rate(rate[i]);
   const float bias = a.dt_bias ? a.dt_bias[dd] : 0.0f, skip = a.D ? a.D[dd] : 0.0f;
 #pragma unroll
   for (int k = 0; k < kStreams; ++k) {
@@ -511,7 +517,7 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
         for (int i = 0; i < 2; ++i) {
           const int n = S::source(lane * kStates + 2 * j + i, states, 1);
           hv[i] = pool && mine_first ? pool[d * states + n] : 0.0f;
-          rv[i] = a.A[d * states + n] * kLog2E;
+          rv[i] = finite_rate(a.A[d * states + n] * kLog2E);
         }
         h[c][j] = pack2(hv[0], hv[1]);
         rate[c][j] = pack2(rv[0], rv[1]);

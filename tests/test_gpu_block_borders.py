@@ -117,3 +117,29 @@ def test_an_infinite_input_without_a_skip(cuda):
         row = slice(t, t + 1)
         y = api.selective_step(d["x"][row], d["dt"][row], d["A"], d["B"][row], d["C"][row], d["state"], None, d["z"][row], d["dt_bias"])
         same_values(y, want[row], bound[row], f"token {t}")
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 32, 37])
+@pytest.mark.parametrize("rate", [-torch.inf, -3.4e38])
+def test_an_infinite_rate_forgets_the_state(cuda, rate, tokens):
+    """A rate of minus infinity (or one that is infinite in base 2) keeps nothing of the state before a token, and the tokens
+    behind a sequence's end, which a tile computes all the same, change nothing."""
+    p = ssm_inputs(tokens, 24, 16, 1, "fp32", 8, 1)
+    p["A"][3, 5] = -1e30
+    want, bound, new, nbound = ssm_reference(p, [0, tokens])
+    p["A"][3, 5] = rate
+    out, state = run_ssm(cuda, p, [0, tokens], None, 0)
+    close(out, want, bound, "y")
+    close(state, new, nbound, "state")
+
+
+@pytest.mark.parametrize("states", [16, 5])
+def test_an_infinite_rate_of_a_single_token(cuda, states):
+    p = ssm_inputs(3, 24, states, 1, "fp32", 8, 3)
+    p["A"][3, 1] = -1e30
+    want, bound, new, nbound = ssm_reference(p, [0, 1, 2, 3])
+    p["A"][3, 1] = -torch.inf
+    d = {k: v.to(cuda) for k, v in p.items()}
+    y = api.selective_step(d["x"], d["dt"], d["A"], d["B"], d["C"], d["state"], d["D"], d["z"], d["dt_bias"])
+    close(y, want, bound, "y")
+    close(d["state"], new, nbound, "state")
