@@ -412,6 +412,13 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int kPending>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
 
+// The state behind a piece: the piece's own, `end`, plus the state h before it times 2^exponent. Token by token an infinite
+// state stays infinite and one of 0 stays 0, so they do here, where the whole piece's factor may be 0 or infinite.
+__device__ __forceinline__ float past_piece(float h, float exponent, float end) {
+  const bool kept = (h == 0.0f || isinf(h)) && isfinite(exponent);
+  return fmaf(kept ? 1.0f : ex2(exponent), h, end);
+}
+
 // The shape of a scan CTA. kLanes lanes hold the states of kPer neighbouring channels, kStates states of each a lane.
 template <typename T, int kLanes_, int kStates_, int kPer_, int kTile_, int kScan_, int kHelpers_, int kCtas_, int kBytes_>
 struct ScanShape {
@@ -625,10 +632,11 @@ __global__ void __launch_bounds__(S::kScan + S::kHelpers, S::kCtas) scan_kernel(
             const f32x2 sums = pack2(sum, sum);
 #pragma unroll
             for (int j = 0; j < kPairs; ++j) {
-              const f32x2 end = pack2(peer(c * (kStates + 1) + 2 * j, q), peer(c * (kStates + 1) + 2 * j + 1, q));
-              float lo, hi;
+              const float end_lo = peer(c * (kStates + 1) + 2 * j, q), end_hi = peer(c * (kStates + 1) + 2 * j + 1, q);
+              float lo, hi, h_lo, h_hi;
               unpack2(mul2(sums, rate[c][j]), lo, hi);
-              h[c][j] = q ? fma2(pack2(ex2(lo), ex2(hi)), h[c][j], end) : end;
+              unpack2(h[c][j], h_lo, h_hi);
+              h[c][j] = q ? pack2(past_piece(h_lo, lo, end_lo), past_piece(h_hi, hi, end_hi)) : pack2(end_lo, end_hi);
             }
           }
       }

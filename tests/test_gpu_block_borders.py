@@ -143,3 +143,26 @@ def test_an_infinite_rate_of_a_single_token(cuda, states):
     y = api.selective_step(d["x"], d["dt"], d["A"], d["B"], d["C"], d["state"], d["D"], d["z"], d["dt_bias"])
     close(y, want, bound, "y")
     close(d["state"], new, nbound, "state")
+
+
+def test_an_infinite_state_across_the_pieces_of_a_split_sequence(cuda):
+    """A state that is infinite stays so, also where its decay over a whole piece is below the smallest number."""
+    p = ssm_inputs(3000, 8, 16, 1, "fp32", 7, 1)
+    p["B"], p["C"], p["dt_bias"] = p["B"].abs() + 0.1, p["C"].abs() + 0.1, torch.full((8,), -1.0)
+    p["x"][100, 2] = torch.inf
+    p["D"] = p["D"].abs() + 0.1
+    want, bound, new, nbound = ssm_reference(p, [0, 3000], pieces=16)
+    assert torch.isinf(new[0, 2]).all()
+    out, state = run_ssm(cuda, p, [0, 3000], None, 0)
+    same_values(out, want, bound, "y")
+    same_values(state, new, nbound, "state")
+
+
+def test_an_empty_state_across_growing_pieces(cuda):
+    """A state of 0 stays 0, also where its growth over a whole piece is above the largest number."""
+    p = ssm_inputs(3000, 8, 16, 1, "fp32", 7, 1)
+    p["A"], p["dt_bias"] = p["A"].abs(), torch.full((8,), 1.0)
+    p["x"].zero_()
+    p["state"].zero_()
+    out, state = run_ssm(cuda, p, [0, 3000], None, 0)
+    assert (out == 0).all() and (state == 0).all()
