@@ -166,3 +166,37 @@ def test_an_empty_state_across_growing_pieces(cuda):
     p["state"].zero_()
     out, state = run_ssm(cuda, p, [0, 3000], None, 0)
     assert (out == 0).all() and (state == 0).all()
+
+
+def reported(call):
+    api.kernel_status()
+    call()
+    with pytest.raises(api.MmfreeError) as e:
+        api.kernel_status()
+    assert e.value.code == _lib.E_RANGE
+    api.kernel_status()
+
+
+@pytest.mark.parametrize("starts,slots", [
+    ([0, 8, 8, 99], None), ([0, 8, 8, 4], None), ([0, 4, 4, 8], [0, 99, 1]), ([8, 8, 8, 8], [0, 1, 99]), ([0, 8, 8, -3], None)])
+def test_bad_sequences_behind_the_last_row_or_empty_are_reported(cuda, starts, slots):
+    """Bounds are checked in the kernels before any access, so these calls end in a status."""
+    p = ssm_inputs(8, 16, 16, 1, "fp32", 3, 3)
+    d = {k: v.to(cuda) for k, v in p.items()}
+    sd = torch.tensor(starts, dtype=torch.int32, device=cuda)
+    sl = None if slots is None else torch.tensor(slots, dtype=torch.int32, device=cuda)
+    reported(lambda: api.selective_scan(d["x"], d["dt"], d["A"], d["B"], d["C"], state=d["state"], seq_starts=sd, slots=sl))
+    for channels in (16, 3):
+        x = d["x"][:, :channels].contiguous()
+        w, st = torch.randn(channels, 4, device=cuda), torch.randn(3, 3, channels, device=cuda)
+        reported(lambda: api.causal_conv(x, w, state=st, seq_starts=sd, slots=sl))
+
+
+@pytest.mark.parametrize("at", [1, 150, 699])
+def test_one_bad_slot_among_many_sequences_is_reported(cuda, at):
+    x, w, st = torch.randn(900, 8, device=cuda), torch.randn(8, 4, device=cuda), torch.randn(700, 3, 8, device=cuda)
+    starts = torch.arange(701, dtype=torch.int32, device=cuda).clamp(max=500)  # the last 200 are empty
+    slots = torch.arange(700, dtype=torch.int32, device=cuda)
+    api.causal_conv(x, w, state=st, seq_starts=starts, slots=slots)
+    slots[at] = 700
+    reported(lambda: api.causal_conv(x, w, state=st, seq_starts=starts, slots=slots))
