@@ -204,7 +204,9 @@ enum { MMFREE_T_F32 = 0, MMFREE_T_BF16 = 1, MMFREE_T_F16 = 2, MMFREE_T_S8 = 3, M
  *   scale = m / (127 or 448) / sqrt(mean(r^2) + eps)
  * x [rows, cols] and residual of `type` (F32, BF16 or F16); codes [rows, cols] and scales
  * [rows, ceil(cols / group)] contiguous; group 0 (one scale a row), 32, 64 or 128. A row of
- * zeros has codes and scale 0; a row with a NaN or an infinity has NaN scales. */
+ * zeros has codes and scale 0, also without an eps; a NaN makes NaN of all scales of its row, an
+ * infinity of its own group's, and 0 of the others (the norm of what is beside it). The mean of
+ * the squares may be outside the range of fp32. */
 int mmfree_cuda_add_rmsnorm_quant(void* codes, float* scales, const void* x, size_t ldx,
                                   void* residual, size_t ld_res, const float* weight,
                                   size_t rows, size_t cols, float eps, int type, int code_type,

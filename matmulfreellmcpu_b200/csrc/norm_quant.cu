@@ -44,18 +44,53 @@ __device__ __forceinline__ void fetch8(const T* p, int n, Words<T, kCols>& w) {
   }
 }
 
+// Whether a row's mean of squares is a number that fp32 holds with all its bits.
+__device__ __forceinline__ bool in_range(float mean) { return mean >= 0x1p-96f && mean <= 3.402823466e38f; }
+
+// The scales of a CTA's rows once more, from sums and products in 64 bits, where the squares are outside fp32's range (values
+// above 1.8e19, a NaN or an infinity) or so small that their rounding counts (without an eps). Behind the last row, where
+// nothing else is live, and not inlined: in the rows' loop, which uses all its registers, it made calls 13 to 24% slower.
+template <typename T>
+__device__ __noinline__ void far_scales(const NormQuantArgs& a, float limit) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __syncthreads();  // the other threads' scales and parts of the residual
+#pragma unroll 1
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* const r = a.residual ? static_cast<const T*>(a.residual) + row * a.ldr : static_cast<const T*>(a.x) + row * a.ldx;
+    double sum = 0.0;  // every warp sums the whole row
+    for (int i = lane; i < a.cols; i += 32) sum += static_cast<double>(to_f32(r[i])) * to_f32(r[i]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    const double mean = sum / a.cols + static_cast<double>(a.eps);
+    // a wider range than in_range's: cols squares, 2^16 at most, may have been out of fp32's where their mean is not
+    if (mean >= 0x1p-95 && mean <= 0x1p110) continue;
+    const double rstd = 1.0 / sqrt(mean);
+    const int group = a.group ? a.group : a.cols;
+    for (int part = warp; part < a.parts; part += blockDim.x >> 5) {
+      uint32_t most = 0;
+      for (int i = part * group + lane; i < min((part + 1) * group, a.cols); i += 32)
+        most = max(most, __float_as_uint(__fmul_rn(to_f32(r[i]), a.weight[i])) & 0x7FFFFFFFu);
+      const double m = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, most));
+      if (lane == 0) a.scales[row * a.parts + part] = mean == 0.0 ? 0.0f : static_cast<float>(m * rstd / limit);
+    }
+  }
+}
+
 // A CTA holds a row in registers, kChunks chunks of 8 columns a thread, and walks the rows with a fixed stride; several
 // small CTAs an SM cover each other's reductions. Two chunks a thread are the best for most rows: 16384 x 2560 bf16 to
 // e4m3 (bound by the issue slots, 60 us, 4.9 TB/s) takes 78 us with one chunk and 75 us with four. Rows of one chunk a
 // thread keep the weights, and where the registers allow it the next row is loaded while this one is reduced and stored
 // (62.9 us without).
 template <typename T, typename Code, int kChunks, bool kVec>
-__global__ void __launch_bounds__(kChunks == 8 ? 896 : 512, kChunks == 8 ? 1 : 2) norm_quant_kernel(NormQuantArgs a) {
+__global__ void __launch_bounds__(kChunks == 8 ? 896 : 512, kChunks == 8 ? 1 : 2) norm_quant_kernel(const __grid_constant__ NormQuantArgs a) {
   constexpr bool kAhead = kChunks * sizeof(T) <= 4, kKeep = kChunks == 1;
   constexpr bool kS8 = std::is_same<Code, int8_t>::value;
   constexpr float kLimit = kS8 ? 127.0f : 448.0f;
   __shared__ __align__(16) float s_sum[2][32];
   __shared__ __align__(16) uint32_t s_most[2][32];
+  __shared__ int s_far;  // whether a row was not in range
+  if (threadIdx.x == 0) s_far = 0;
+  __syncthreads();
   const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5;
   const bool add = a.residual != nullptr;
   const int parts_shift = a.group ? __ffs(a.group) - 1 : 0;
@@ -149,7 +184,9 @@ __global__ void __launch_bounds__(kChunks == 8 ? 896 : 512, kChunks == 8 ? 1 : 2
         for (int i = 0; i < warps; ++i) row_most = max(row_most, s_most[buf][i]);
       }
     }
-    const float rstd = rsqrtf(fmaf(sum, inv_cols, a.eps));
+    const float mean = fmaf(sum, inv_cols, a.eps);
+    const float rstd = rsqrtf(mean);
+    if (!in_range(mean)) s_far = 1;
     float* const scales = a.scales + row * a.parts;
     if (a.group == 0 && tid == 0) scales[0] = __uint_as_float(row_most) * rstd * (1.0f / kLimit);
 #pragma unroll
@@ -189,6 +226,8 @@ __global__ void __launch_bounds__(kChunks == 8 ? 896 : 512, kChunks == 8 ? 1 : 2
       }
     }
   }
+  __syncthreads();
+  if (s_far) far_scales<T>(a, kLimit);
 }
 
 template <typename T, typename Code, int kChunks, bool kVec>

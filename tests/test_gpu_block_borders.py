@@ -9,7 +9,7 @@ import torch
 
 import block_ref as R
 from matmulfreellmcpu_b200 import _lib, api
-from test_gpu_block_ops import SENTINEL, close, rng, run_ssm, ssm_inputs
+from test_gpu_block_ops import SENTINEL, close, rng, run_ssm, sliced, ssm_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -200,3 +200,60 @@ def test_one_bad_slot_among_many_sequences_is_reported(cuda, at):
     api.causal_conv(x, w, state=st, seq_starts=starts, slots=slots)
     slots[at] = 700
     reported(lambda: api.causal_conv(x, w, state=st, seq_starts=starts, slots=slots))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("group", [0, 32])
+@pytest.mark.parametrize("kind,cols,extra", [("fp32", 96, 0), ("bf16", 2560, 0), ("bf16", 100, 3), ("fp32", 8192, 0), ("fp16", 96, 0)])
+def test_norm_scales_of_very_large_and_very_small_rows(cuda, kind, cols, extra, group, code):
+    """The squares of these rows are out of fp32's range; their scales are not."""
+    g = rng(cols)
+    sizes = torch.tensor([1.0, 1e30, 2e37, 1e-25, 1e-30, 1e-39, 1.0, 3e18, 1e-18])
+    if kind == "fp16":
+        sizes = torch.tensor([1.0, 1e3, 1e4, 1e-3, 1e-4, 1e-6, 1.0, 8e3, 1e-5])
+    x = (torch.randn(9, cols, generator=g) * sizes[:, None]).to(R.TYPES[kind])
+    res = (torch.randn(9, cols, generator=g) * sizes[:, None]).to(R.TYPES[kind])
+    w = 0.25 + torch.rand(cols, generator=g) / 2
+    for eps in (0.0, 1e-6, 1e-30):
+        for residual in (None, res):
+            q, s, r = R.norm_quant_ref(x, w, residual, eps, code, group)
+            rd = None if residual is None else sliced(residual, extra, cuda)
+            gq, gs = api.add_rmsnorm_quant(sliced(x, extra, cuda), w.to(cuda), rd, eps, code, group)
+            # as test_norm_quant, and half a step of the smallest numbers
+            close(gs, s, s * (cols / 2 + 6) * R.U + 2.0 ** -149, f"scales, eps {eps}")
+            if code == "int8":
+                assert torch.equal(gq.cpu(), q)
+            if residual is not None:
+                assert torch.equal(rd.cpu(), r)
+
+
+@pytest.mark.parametrize("group", [0, 32])
+def test_norm_of_a_zero_row_without_eps(cuda, group):
+    x = torch.randn(3, 96, generator=rng(1))
+    x[1] = 0
+    q, s = api.add_rmsnorm_quant(x.to(cuda), torch.ones(96, device=cuda), eps=0.0, group=group)
+    assert (q[1] == 0).all() and (s[1] == 0).all() and (s[[0, 2]] > 0).all() and torch.isfinite(s).all()
+
+
+def test_norm_of_a_row_with_an_infinity(cuda):
+    """The norm of an infinity is a NaN, of everything beside it 0."""
+    x = torch.randn(1, 96, generator=rng(1))
+    x[0, 40] = -torch.inf
+    q, s = api.add_rmsnorm_quant(x.to(cuda), torch.ones(96, device=cuda), group=32)
+    assert torch.isnan(s[0, 1]) and (s[0, [0, 2]] == 0).all()
+
+
+@pytest.mark.parametrize("group", [0, 128])
+def test_norm_of_many_rows_of_which_some_are_far(cuda, group):
+    """More rows than the device holds at once, far ones among them, and rows whose every value is a NaN."""
+    rows, cols = 3000, 1500
+    x = torch.randn(rows, cols, generator=rng(5))
+    far = torch.tensor([0, 1, 700, 1999, 2999])
+    x[far] *= torch.tensor([1e25, 1e-25, 1e30, 1e-30, 1e37])[:, None]
+    x[1234] = torch.nan
+    w = 0.5 + torch.rand(cols, generator=rng(6)) / 2
+    q, s, _ = R.norm_quant_ref(x, w, None, 0.0, "int8", group)
+    gq, gs = api.add_rmsnorm_quant(x.to(cuda), w.to(cuda), eps=0.0, group=group)
+    rest = [i for i in range(rows) if i != 1234]
+    assert torch.equal(gq.cpu()[rest], q[rest]) and torch.isnan(gs[1234]).all()
+    close(gs[rest], s[rest], s[rest] * (cols / 2 + 6) * R.U, "scales")
