@@ -220,8 +220,7 @@ int mmfree_cuda_add_rmsnorm_quant(void* codes, float* scales, const void* x, siz
  * or F16 with x_scales NULL, or S8 / E4M3 codes with the scales of
  * mmfree_cuda_add_rmsnorm_quant: x_scales [rows] with x_group 0, or [rows, ceil(in_dim /
  * group)] with x_group == group. out [rows, out_dim] contiguous of out_type (F32, BF16 or
- * F16). Sums are in fp32 (whole numbers within a group for S8 rows); an F32 row with an infinity
- * gives NaN. Meant for a few rows (1 to 32), right for any number. */
+ * F16). Sums are in fp32 (whole numbers within a group for S8 rows). Meant for a few rows (1 to 32), right for any number. */
 int mmfree_cuda_int4_matvec(void* out, const void* x, size_t ldx, const float* x_scales,
                             const uint8_t* codes, size_t ld_codes, const void* scales,
                             const uint8_t* zeros, size_t rows, size_t in_dim, size_t out_dim,

@@ -375,8 +375,7 @@ def int4_matvec(x, codes, scales, group: int, zeros=None, x_scales=None, out_dty
     uint8 of that shape (at most 127). ``x`` [rows, in_dim] float32, bfloat16 or float16, or the int8 or e4m3
     codes of :func:`add_rmsnorm_quant` with its scales as ``x_scales`` (one a row, or of the
     same ``group``). Returns [rows, out_dim] of ``out_dtype`` (``x``'s type; float32 for codes).
-    Row pitches of ``codes`` that are multiples of 16 bytes are the fast ones. A float32 row with
-    an infinity gives NaN."""
+    Row pitches of ``codes`` that are multiples of 16 bytes are the fast ones."""
     return bind().int4_matvec(x, codes, scales, group, zeros, x_scales, out_dtype, stream)
 
 

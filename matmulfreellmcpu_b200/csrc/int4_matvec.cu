@@ -181,8 +181,40 @@ struct Int4Shape {
   struct Shared {
     Warp warp[kWarps];
     float part[kWarps][kCols][kPitch];
+    int nan;  // fp32 rows: whether an output was one
   };
 };
+
+__device__ __forceinline__ float get_out(const void* p, int type, int64_t i) {
+  switch (type) {
+    case MMFREE_T_F32: return static_cast<const float*>(p)[i];
+    case MMFREE_T_BF16: return to_f32(static_cast<const __nv_bfloat16*>(p)[i]);
+    default: return to_f32(static_cast<const __half*>(p)[i]);
+  }
+}
+
+// Outputs of fp32 rows that came out as NaN, once more from the definition in 64 bits, each by the thread that stored it. An
+// infinity's first part is the infinity and its second infinity minus infinity, so its row's outputs are all NaN at first;
+// telling it apart where rows are cut cost every call 8 to 19%.
+__device__ __noinline__ void nan_outputs(const Int4Args& a, int splits, int m0, int live) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.x % splits;
+  for (int64_t n = static_cast<int64_t>(blockIdx.x / splits) * 32 + lane; n < a.N; n += static_cast<int64_t>(gridDim.x / splits) * 32)
+    for (int m = rank * kWarps + warp; m < live; m += splits * kWarps) {
+      const int64_t at = static_cast<int64_t>(m0 + m) * a.N + n;
+      if (!isnan(get_out(a.out, a.out_type, at))) continue;
+      const float* const x = static_cast<const float*>(a.x) + static_cast<int64_t>(m0 + m) * a.ldx;
+      const uint8_t* const codes = a.codes + n * a.ldw;
+      double total = 0.0;
+      for (int g = 0; g < a.parts; ++g) {
+        const int64_t of = n * a.parts + g;
+        const int zero = a.zeros ? a.zeros[of] : 8, stop = min(static_cast<int64_t>(a.K), (g + int64_t(1)) * a.group);
+        double part = 0.0;
+        for (int k = g * a.group; k < stop; ++k) part += static_cast<double>((codes[k >> 1] >> (4 * (k & 1)) & 15) - zero) * x[k];
+        total += part * get_out(a.scales, a.scale_type, of);
+      }
+      put_out(a.out, a.out_type, at, static_cast<float>(total));
+    }
+}
 
 // A CTA: 32 weight rows and 8 * kTiles activation rows at a time; its warps (and those of the other CTAs of its
 // cluster) split the columns into turns of kTileK. The row blocks are walked by a fixed grid.
@@ -190,7 +222,7 @@ struct Int4Shape {
 // touches are copied (a chunk with a byte of the row in it can be read as a whole) and its words put together from
 // two, shifted by the row's own offset.
 template <int kType, int kTiles, bool kAligned>
-__global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCtas) int4_kernel(Int4Args a, int splits, int m0, bool xvec, uint32_t group_inverse) {
+__global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCtas) int4_kernel(const __grid_constant__ Int4Args a, int splits, int m0, bool xvec, uint32_t group_inverse) {
   using X = RowType<kType>;
   using S = Int4Shape<kTiles, kAligned>;
   constexpr int kBlocks = S::kBlocks, kRows = S::kRows, kCols = S::kCols, kChunks = S::kChunks, kStages = S::kStages;
@@ -203,6 +235,8 @@ __global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCta
   const int stride = kWarps * splits, first = rank * kWarps + warp;
   const int live = min(kCols, a.M - m0);
   const char* const x = static_cast<const char*>(a.x) + static_cast<int64_t>(m0) * a.ldx * X::kBytes;
+
+  if (kType == MMFREE_T_F32 && threadIdx.x == 0) sh.nan = 0;  // set behind the first block's barrier
 
   // k / group: columns are below 2^16, where the high word of the product with ceil(2^32 / group) is exact
   const auto group_of = [&](int k) { return static_cast<int>(__umulhi(static_cast<uint32_t>(k), group_inverse)); };
@@ -409,6 +443,7 @@ __global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCta
     const auto put = [&](int m, float v) {
       const int n = block * kRows + lane;
       if (m >= live || n >= a.N) return;
+      if (kType == MMFREE_T_F32 && isnan(v)) sh.nan = 1;
       if (a.x_scales && !a.x_grouped) v *= a.x_scales[m0 + m];
       put_out(a.out, a.out_type, static_cast<int64_t>(m0 + m) * a.N + n, v);
     };
@@ -440,6 +475,8 @@ __global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCta
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if constexpr (kType == MMFREE_T_F32)
+    if (sh.nan) nan_outputs(a, splits, m0, live);  // set before the last block's barrier
 }
 
 template <int kType, int kTiles, bool kAligned>

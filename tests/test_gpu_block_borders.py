@@ -9,7 +9,7 @@ import torch
 
 import block_ref as R
 from matmulfreellmcpu_b200 import _lib, api
-from test_gpu_block_ops import SENTINEL, close, rng, run_ssm, sliced, ssm_inputs
+from test_gpu_block_ops import SENTINEL, close, dev, int4_inputs, rng, run_ssm, sliced, ssm_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -257,3 +257,33 @@ def test_norm_of_many_rows_of_which_some_are_far(cuda, group):
     rest = [i for i in range(rows) if i != 1234]
     assert torch.equal(gq.cpu()[rest], q[rest]) and torch.isnan(gs[1234]).all()
     close(gs[rest], s[rest], s[rest] * (cols / 2 + 6) * R.U, "scales")
+
+
+@pytest.mark.parametrize("k", [300, 512])
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "fp16"])
+def test_int4_matvec_infinities(cuda, kind, k):
+    x, codes, scales, _, _ = int4_inputs(4, k, 40, 64, False, kind, 11)
+    x[1, 17] = torch.inf
+    x[2, 200], x[2, 3] = -torch.inf, torch.inf
+    want, bound = R.int4_ref(x, codes, scales, 64)
+    want[torch.isnan(want)] = torch.nan
+    out = api.int4_matvec(*dev(cuda, x, codes, scales), 64)
+    same_values(out, want, bound + R.rounding(want, out.dtype), kind)
+
+
+def test_int4_matvec_a_nan_of_low_bits_only(cuda):
+    """The NaN whose upper half is that of an infinity."""
+    x, codes, scales, _, _ = int4_inputs(2, 512, 40, 64, False, "fp32", 11)
+    x.view(torch.int32)[1, 9] = 0x7F800001
+    out = api.int4_matvec(*dev(cuda, x, codes, scales), 64)
+    assert torch.isnan(out[1]).all() and torch.isfinite(out[0]).all()
+
+
+@pytest.mark.parametrize("m,k,n,extra,out_type", [(9, 5632, 160, 0, torch.float32), (2, 320, 9700, 1, torch.bfloat16), (20, 321, 5000, 0, torch.float16)])
+def test_int4_matvec_infinities_of_split_and_of_many_rows(cuda, m, k, n, extra, out_type):
+    x, codes, scales, z, _ = int4_inputs(m, k, n, 64, True, "fp32", 12)
+    scales = scales * 0.01
+    x[1, k // 2], x[m - 1, 3] = -torch.inf, torch.nan
+    want, bound = R.int4_ref(x, codes, scales, 64, z)
+    out = api.int4_matvec(x.to(cuda), sliced(codes, extra, cuda), scales.to(cuda), 64, zeros=z.to(cuda), out_dtype=out_type)
+    same_values(out, want, bound + R.rounding(want, out_type), f"{m} x {k} -> {n}")
