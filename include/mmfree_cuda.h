@@ -73,14 +73,13 @@ int mmfree_cuda_bitlinear(float* out, const float* x, const float* norm_weight,
                           int frac_bits, int32_t* acc_out, void* stream);
 
 /* Status of the asynchronous kernel entry points (mmfree_cuda_bitlinear,
- * mmfree_cuda_bitlinear_cluster, mmfree_cuda_bitlinear_noalloc, mmfree_cuda_causal_conv,
- * mmfree_cuda_selective_scan and their steps). They return once their
- * kernels are queued; a failure inside a kernel (a bounded wait that gave up, a sequence
- * start or slot out of range) is recorded in
- * a device error word instead. This call synchronizes `stream` (the stream those calls used),
+ * mmfree_cuda_bitlinear_cluster, mmfree_cuda_bitlinear_noalloc, mmfree_cuda_int4_matvec,
+ * mmfree_cuda_causal_conv, mmfree_cuda_selective_scan and their steps). They return once their
+ * kernels are queued; a failure inside a kernel (a bounded wait that gave up, a sequence start,
+ * slot or zero point out of range) is recorded in a device error word instead. This call synchronizes `stream` (the stream those calls used),
  * reads and clears the calling device's words and returns MMFREE_OK, or MMFREE_E_TIMEOUT when
  * a call since the last check failed -- the outputs of those calls are then undefined -- or
- * MMFREE_E_RANGE when one met a bad sequence start or slot. It
+ * MMFREE_E_RANGE when one met a bad sequence start, slot or zero point. It
  * allocates nothing. No reference counterpart: the reference kernels are synchronous host
  * code that cannot time out. */
 int mmfree_cuda_kernel_status(void* stream);
@@ -215,8 +214,10 @@ int mmfree_cuda_add_rmsnorm_quant(void* codes, float* scales, const void* x, siz
 /* out[m, n] = x_scales[m] * sum_k x[m, k] * (u[n, k] - zero[n, k / group]) * scale[n, k / group]
  * for 4-bit weights u in 0..15. codes: [out_dim, ceil(in_dim / 2)] bytes with row pitch
  * ld_codes bytes, element 2j in the low and 2j + 1 in the high half of byte j; scales
- * [out_dim, ceil(in_dim / group)] of scale_type (F32, BF16 or F16) and zeros (uint8 of at
- * most 127, same shape; NULL: 8) contiguous; group a multiple of 32. x [rows, in_dim] of x_type: F32, BF16
+ * [out_dim, ceil(in_dim / group)] of scale_type (F32, BF16 or F16) and zeros (uint8, same
+ * shape; NULL: 8) contiguous; group a multiple of 32. For F32 and BF16 rows a zero point is 127
+ * at most: one above makes the outputs of its weight row wrong and is recorded
+ * (mmfree_cuda_kernel_status returns MMFREE_E_RANGE). x [rows, in_dim] of x_type: F32, BF16
  * or F16 with x_scales NULL, or S8 / E4M3 codes with the scales of
  * mmfree_cuda_add_rmsnorm_quant: x_scales [rows] with x_group 0, or [rows, ceil(in_dim /
  * group)] with x_group == group. out [rows, out_dim] contiguous of out_type (F32, BF16 or

@@ -274,7 +274,9 @@ def nccl_unique_id() -> bytes:
 def kernel_status(stream=None) -> None:
     """Synchronizes ``stream`` and raises MmfreeError (code E_TIMEOUT) when a kernel of an
     asynchronous entry point (bitlinear, bitlinear_cluster, bitlinear_noalloc) gave up a
-    bounded wait since the last check; the recorded error is cleared."""
+    bounded wait since the last check, or (code E_RANGE) one of causal_conv, selective_scan, their
+    steps and int4_matvec met a sequence start, slot or zero point out of range; the recorded error
+    is cleared."""
     check(lib().mmfree_cuda_kernel_status(_stream(stream)))
 
 
@@ -372,7 +374,8 @@ def int4_matvec(x, codes, scales, group: int, zeros=None, x_scales=None, out_dty
 
     ``codes`` uint8 [out_dim, ceil(in_dim / 2)], two weights a byte, the even column's in the
     low half; ``scales`` [out_dim, ceil(in_dim / group)] float32, bfloat16 or float16; ``zeros``
-    uint8 of that shape (at most 127). ``x`` [rows, in_dim] float32, bfloat16 or float16, or the int8 or e4m3
+    uint8 of that shape (at most 127 for float32 and bfloat16 rows; one above is reported by
+    :func:`kernel_status`). ``x`` [rows, in_dim] float32, bfloat16 or float16, or the int8 or e4m3
     codes of :func:`add_rmsnorm_quant` with its scales as ``x_scales`` (one a row, or of the
     same ``group``). Returns [rows, out_dim] of ``out_dtype`` (``x``'s type; float32 for codes).
     Row pitches of ``codes`` that are multiples of 16 bytes are the fast ones."""

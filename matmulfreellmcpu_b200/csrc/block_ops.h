@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/mmfree_cuda.h"
@@ -37,9 +38,38 @@ struct Int4Args {
 };
 cudaError_t launch_int4_matvec(const Int4Args& a, int sm_count, cudaStream_t s);
 
-// The sequence errors of causal_conv and selective_scan (kErrRange) since the last call, read
-// on `s` (synchronizing it) and cleared; 0 when no such kernel was launched on this device.
+// The errors (kErrRange) of causal_conv and selective_scan (sequence starts and slots) and of
+// int4_matvec (zero points) since the last call, read on `s` (synchronizing it) and cleared; 0
+// when no such kernel was launched on this device.
 cudaError_t take_sequence_flags(cudaStream_t s, uint32_t* flags);
+cudaError_t take_zero_point_flags(cudaStream_t s, uint32_t* flags);
+
+// The devices on which a file's kernels were launched.
+class LaunchedOn {
+ public:
+  void mark() {
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess) bits_.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_relaxed);
+  }
+  bool has(int dev) const { return bits_.load(std::memory_order_relaxed) >> (dev & 63) & 1; }
+
+ private:
+  std::atomic<uint64_t> bits_{0};
+};
+
+// Reads and clears a __device__ error word of the calling device on `s`, synchronizing it.
+inline cudaError_t take_word(uint32_t& symbol, const LaunchedOn& devices, cudaStream_t s, uint32_t* flags) {
+  *flags = 0;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || !devices.has(dev)) return e;
+  e = cudaMemcpyFromSymbolAsync(flags, symbol, 4, 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess || !*flags) return e;
+  const uint32_t zero = 0;
+  e = cudaMemcpyToSymbolAsync(symbol, &zero, 4, 0, cudaMemcpyHostToDevice, s);
+  return e == cudaSuccess ? cudaStreamSynchronize(s) : e;
+}
 
 cudaError_t launch_causal_conv(const mmfree_cuda_conv_args& a, cudaStream_t s);
 cudaError_t launch_causal_conv_step(const mmfree_cuda_conv_args& a, cudaStream_t s);

@@ -417,12 +417,16 @@ int mmfree_cuda_kernel_status(void* stream) {
     }
     if (arena) f |= take_flags(reinterpret_cast<uint32_t*>(arena) + kAsyncFlagWord, st);
     if (char* head = noalloc_base_if_ready(dev)) f |= take_flags(reinterpret_cast<uint32_t*>(head), st);
-    uint32_t sequence = 0;
+    uint32_t sequence = 0, zero_point = 0;
     ck(take_sequence_flags(st, &sequence), "reading the sequence error word");
-    f |= sequence;
+    ck(take_zero_point_flags(st, &zero_point), "reading the zero point error word");
+    f |= sequence | zero_point;
     if (f & kErrTimeout)
       throw TimeoutError("a bounded wait inside a BitLinear kernel gave up: the outputs of the "
                          "kernel calls since the last status check are undefined");
+    if (zero_point & kErrRange)
+      throw std::out_of_range("a zero point given to int4_matvec with F32 or BF16 rows since the "
+                              "last status check is above 127");
     if (f & kErrRange)
       throw std::out_of_range("a sequence start or slot given to causal_conv or selective_scan "
                               "since the last status check is out of range or out of order");

@@ -30,7 +30,12 @@
 
 namespace mmfree_cuda {
 
+// Bit kErrRange once a zero point was above 127 for rows that become bf16 operands.
+__device__ uint32_t g_zero_point_error;
+
 namespace {
+
+LaunchedOn g_devices;
 
 constexpr int kWarps = 8;       // of a CTA: they share its weight rows and split the columns
 constexpr int kTileK = 256;     // columns of a warp's turn (128 bytes of a weight row)
@@ -295,7 +300,8 @@ __global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCta
       if (i >= next_groups) break;
       mine.scale[i][lane] = a.scale_type == MMFREE_T_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(next_scale[i])))
                                                          : __uint_as_float(next_scale[i] << (wide_scales ? 0 : 16));
-      // 128 + z or 1024 + z twice (z up to 127 is exact): 0x4300 + z is 128 + z in bf16, 0x6400 + z is 1024 + z in fp16
+      if (X::kBf16 && next_zero[i] > 127) atomicOr(&g_zero_point_error, kErrRange);
+      // 128 + z (up to z = 127 exact) or 1024 + z twice: 0x4300 + z is 128 + z in bf16, 0x6400 + z is 1024 + z in fp16
       mine.zero[i][lane] = (X::kBf16 ? 0x43004300u : 0x64006400u) + next_zero[i] * 0x10001u;
     }
   };
@@ -530,7 +536,10 @@ cudaError_t int4_type(const Int4Args& a, int sms, cudaStream_t s) {
 
 }  // namespace
 
+cudaError_t take_zero_point_flags(cudaStream_t s, uint32_t* flags) { return take_word(g_zero_point_error, g_devices, s, flags); }
+
 cudaError_t launch_int4_matvec(const Int4Args& a, int sm_count, cudaStream_t s) {
+  g_devices.mark();
   switch (a.x_type) {
     case MMFREE_T_F32: return int4_type<MMFREE_T_F32>(a, sm_count, s);
     case MMFREE_T_BF16: return int4_type<MMFREE_T_BF16>(a, sm_count, s);

@@ -10,7 +10,6 @@
 #include "elements.cuh"
 #include "tcgen05.cuh"
 
-#include <atomic>
 #include <type_traits>
 
 namespace mmfree_cuda {
@@ -20,12 +19,7 @@ __device__ uint32_t g_sequence_error;
 
 namespace {
 
-std::atomic<uint64_t> g_devices{0};  // devices on which one of these kernels was launched
-
-void mark_device() {
-  int dev = 0;
-  if (cudaGetDevice(&dev) == cudaSuccess) g_devices.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_relaxed);
-}
+LaunchedOn g_devices;
 
 __device__ __forceinline__ void sequence_error() { atomicOr(&g_sequence_error, kErrRange); }
 
@@ -230,7 +224,7 @@ __global__ void __launch_bounds__(128) conv_step_kernel(mmfree_cuda_conv_args a)
 template <typename T, int W, int V>
 cudaError_t conv_launch(const mmfree_cuda_conv_args& a, bool step, cudaStream_t s) {
   const unsigned blocks = static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.channels), 128 * V));
-  mark_device();
+  g_devices.mark();
   if (step) return launch_k(conv_step_kernel<T, W, V>, dim3(blocks, static_cast<unsigned>(a.seqs)), dim3(128), 0, s, false, a);
   // Tokens of a tile: 64, before which W - 1 are read once more (16384 x 5120 bf16: 68 us; 76 us with tiles of 128),
   // fewer where the tiles would not fill the 148 SMs (300 x 2048: 8.0 us, 14.6 us with 64).
@@ -916,7 +910,7 @@ cudaError_t step_type(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
 }
 
 cudaError_t step_any(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
-  mark_device();
+  g_devices.mark();
   switch (a.type) {
     case MMFREE_T_F32: return step_type<float>(a, s);
     case MMFREE_T_BF16: return step_type<__nv_bfloat16>(a, s);
@@ -925,7 +919,7 @@ cudaError_t step_any(const mmfree_cuda_ssm_args& a, cudaStream_t s) {
 }
 
 cudaError_t scan_any(const mmfree_cuda_ssm_args& a, int sms, cudaStream_t s) {
-  mark_device();
+  g_devices.mark();
   switch (a.type) {
     case MMFREE_T_F32: return scan_type<float>(a, sms, s);
     case MMFREE_T_BF16: return scan_type<__nv_bfloat16>(a, sms, s);
@@ -935,18 +929,7 @@ cudaError_t scan_any(const mmfree_cuda_ssm_args& a, int sms, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t take_sequence_flags(cudaStream_t s, uint32_t* flags) {
-  *flags = 0;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess || !(g_devices.load(std::memory_order_relaxed) >> (dev & 63) & 1)) return e;
-  e = cudaMemcpyFromSymbolAsync(flags, g_sequence_error, 4, 0, cudaMemcpyDeviceToHost, s);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-  if (e != cudaSuccess || !*flags) return e;
-  const uint32_t zero = 0;
-  e = cudaMemcpyToSymbolAsync(g_sequence_error, &zero, 4, 0, cudaMemcpyHostToDevice, s);
-  return e == cudaSuccess ? cudaStreamSynchronize(s) : e;
-}
+cudaError_t take_sequence_flags(cudaStream_t s, uint32_t* flags) { return take_word(g_sequence_error, g_devices, s, flags); }
 
 cudaError_t launch_causal_conv(const mmfree_cuda_conv_args& a, cudaStream_t s) { return conv_any(a, false, s); }
 cudaError_t launch_causal_conv_step(const mmfree_cuda_conv_args& a, cudaStream_t s) { return conv_any(a, true, s); }

@@ -287,3 +287,36 @@ def test_int4_matvec_infinities_of_split_and_of_many_rows(cuda, m, k, n, extra, 
     want, bound = R.int4_ref(x, codes, scales, 64, z)
     out = api.int4_matvec(x.to(cuda), sliced(codes, extra, cuda), scales.to(cuda), 64, zeros=z.to(cuda), out_dtype=out_type)
     same_values(out, want, bound + R.rounding(want, out_type), f"{m} x {k} -> {n}")
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "fp16", "int8", "e4m3"])
+@pytest.mark.parametrize("n", [40, 20000])
+def test_int4_matvec_zero_points(cuda, kind, n):
+    """Zero points are exact, up to 127 where rows become bf16 operands; there one above is reported."""
+    g = rng(n)
+    limited = kind in ("fp32", "bf16")
+    most = 127 if limited else 255
+    codes = torch.randint(0, 256, (n, 128), generator=g, dtype=torch.uint8)
+    scales = torch.ldexp(torch.ones(n, 4), torch.randint(-2, 3, (n, 4), generator=g))
+    zeros = torch.randint(0, most + 1, (n, 4), generator=g, dtype=torch.uint8)
+    zeros[0, 0] = zeros[n - 1, 3] = most
+    x = torch.randint(-4, 5, (2, 256), generator=g).float()
+    xs = None
+    if kind in R.TYPES:
+        x = x.to(R.TYPES[kind])
+    else:
+        x, xs = x.to(torch.int8 if kind == "int8" else torch.float8_e4m3fn), torch.ones(2, 1)
+    want, _ = R.int4_ref(x, codes, scales, 64, zeros, xs)  # whole numbers of at most 2^20 quarters: exact in any order
+    xd, cd, sd, zd, xsd = dev(cuda, x, codes, scales, zeros, xs)
+    api.kernel_status()
+    out = api.int4_matvec(xd, cd, sd, 64, zeros=zd, x_scales=xsd, out_dtype=torch.float32)
+    assert torch.equal(out.double().cpu(), want)
+    api.kernel_status()
+    for row, part in ((n - 1, 3), (n // 2, 1)) if limited else ():
+        bad = zd.clone()
+        bad[row, part] = 128
+        api.int4_matvec(xd, cd, sd, 64, zeros=bad, x_scales=xsd)
+        with pytest.raises(api.MmfreeError) as e:
+            api.kernel_status()
+        assert e.value.code == _lib.E_RANGE and "zero point" in str(e.value)
+        api.kernel_status()
