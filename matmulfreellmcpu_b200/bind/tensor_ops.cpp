@@ -105,6 +105,11 @@ struct Arg {
     for (int64_t d = 0; d < t->dim(); ++d) last += (t->size(d) - 1) * t->stride(d);
     return {b, b + (last + 1) * static_cast<int64_t>(t->element_size())};
   }
+  // A call has written the tensor: a graph that saved it must not use it any more. (Tensors made in inference mode have no
+  // versions.)
+  void written() const {
+    if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  }
   void apart(const Arg& o) const {
     if (!o) return;
     const auto a = span(), b = o.span();
@@ -225,6 +230,7 @@ PyObject* add_rmsnorm_quant(PyObject* const* v) {
   check(mmfree_cuda_add_rmsnorm_quant(codes.data_ptr(), static_cast<float*>(scales.data_ptr()), x.data(), ldx, residual.data(), ldr,
                                       static_cast<const float*>(weight.data()), rows, cols, static_cast<float>(eps), kind,
                                       s8 ? MMFREE_T_S8 : MMFREE_T_E4M3, group, on.raw()));
+  residual.written();
   return Py_BuildValue("NN", THPVariable_Wrap(codes), THPVariable_Wrap(scales));
 }
 
@@ -314,6 +320,8 @@ PyObject* causal_conv(PyObject* const* v) {
   a.silu = truth(v[6]);
   on.hold({&x, &weight, &bias, &state, &starts, &slots, &given});
   check(step ? mmfree_cuda_causal_conv_step(&a, on.raw()) : mmfree_cuda_causal_conv(&a, on.raw()));
+  state.written();
+  given.written();
   return THPVariable_Wrap(out);
 }
 
@@ -385,6 +393,8 @@ PyObject* selective(PyObject* const* v) {
   a.dt_softplus = truth(v[8]);
   on.hold({&x, &dt, &A, &B, &Cm, &D, &z, &dt_bias, &state, &starts, &slots, &given});
   check(step ? mmfree_cuda_selective_step(&a, on.raw()) : mmfree_cuda_selective_scan(&a, on.raw()));
+  state.written();
+  given.written();
   return THPVariable_Wrap(out);
 }
 

@@ -320,3 +320,31 @@ def test_int4_matvec_zero_points(cuda, kind, n):
             api.kernel_status()
         assert e.value.code == _lib.E_RANGE and "zero point" in str(e.value)
         api.kernel_status()
+
+
+def test_tensors_written_in_place_get_a_new_version(cuda):
+    """A graph that saved a tensor which a call then overwrites refuses its backward pass."""
+    x, w = torch.randn(4, 16, device=cuda), torch.randn(16, 4, device=cuda)
+    p = {k: v.to(cuda) for k, v in ssm_inputs(4, 16, 4, 1, "fp32", 3, 4).items()}
+
+    def written(t, call):
+        leaf = torch.ones_like(t, requires_grad=True)
+        before, loss = t._version, (leaf * t).sum()  # the product keeps t for leaf's gradient
+        call()
+        assert t._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+    res, st, out = torch.randn(4, 16, device=cuda), torch.randn(4, 3, 16, device=cuda), torch.empty(4, 16, device=cuda)
+    written(res, lambda: api.add_rmsnorm_quant(x, torch.ones(16, device=cuda), res))
+    written(st, lambda: api.causal_conv(x, w, state=st))
+    written(st, lambda: api.causal_conv_step(x, w, st))
+    written(out, lambda: api.causal_conv(x, w, out=out))
+    scan = (p["x"], p["dt"], p["A"], p["B"], p["C"])
+    written(p["state"], lambda: api.selective_scan(*scan, state=p["state"]))
+    written(p["state"], lambda: api.selective_step(*scan, p["state"]))
+    written(out, lambda: api.selective_scan(*scan, out=out))
+    with torch.inference_mode():  # tensors without versions
+        state = torch.zeros(4, 3, 16, device=cuda)
+        api.causal_conv_step(x, w, state)
+    api.causal_conv_step(x, w, state)
