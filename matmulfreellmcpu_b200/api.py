@@ -352,7 +352,8 @@ def rmsnorm_swishgate(g, o, weight, eps: float = 1e-6, stream=None):
 # call runs on that stream and its outputs belong to it, as torch tensors made under
 # ``torch.cuda.stream(stream)`` do; without, on the current stream of the tensors' device.
 # bind/tensor_ops.cpp checks the tensors and makes the outputs. There is no backward pass: an
-# input that requires a gradient is refused while gradients are recorded.
+# input that requires a gradient is refused while gradients are recorded, one with a forward-mode
+# tangent always.
 
 def add_rmsnorm_quant(x, weight, residual=None, eps: float = 1e-6, code: str = "int8", group: int = 0,
                       stream=None):

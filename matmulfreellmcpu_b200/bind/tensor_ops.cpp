@@ -6,6 +6,7 @@
 // times as long as the kernel of one token. matmulfreellmcpu_b200/api.py documents the functions.
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -69,6 +70,8 @@ struct Arg {
     if (t->layout() != at::kStrided) refuse(std::string(n) + " must be a strided tensor");
     if (t->requires_grad() && at::GradMode::is_enabled())
       refuse(std::string(n) + " requires a gradient, and this operator has no backward pass");
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined())
+      refuse(std::string(n) + " has a tangent, and this operator has no forward-mode gradient");
   }
   explicit operator bool() const { return t != nullptr; }
   void* data() const { return t ? t->data_ptr() : nullptr; }

@@ -348,3 +348,14 @@ def test_tensors_written_in_place_get_a_new_version(cuda):
         state = torch.zeros(4, 3, 16, device=cuda)
         api.causal_conv_step(x, w, state)
     api.causal_conv_step(x, w, state)
+
+
+def test_forward_mode_tangents_are_refused(cuda):
+    import torch.autograd.forward_ad as fw
+    x, w = torch.randn(4, 16, device=cuda), torch.randn(16, 4, device=cuda)
+    with fw.dual_level():
+        for with_grad in (True, False):
+            with torch.set_grad_enabled(with_grad), pytest.raises(api.MmfreeError) as e:
+                api.causal_conv(fw.make_dual(x, torch.ones_like(x)), w)
+            assert e.value.code == _lib.E_INVALID and "gradient" in str(e.value)
+        api.causal_conv(x, w)
