@@ -113,10 +113,29 @@ struct Arg {
   void written() const {
     if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   }
+  // Bytes of a row (all dimensions but the first), or 0 where a row has gaps.
+  int64_t row_bytes() const {
+    int64_t n = 1;
+    for (int64_t d = t->dim() - 1; d > 0; --d) {
+      if (t->size(d) > 1 && t->stride(d) != n) return 0;
+      n *= t->size(d);
+    }
+    return n * static_cast<int64_t>(t->element_size());
+  }
+  // Whether the tensors, whose starts are `offset` bytes apart, are different columns of rows with one pitch (two slices of
+  // a wider buffer): their spans overlap, but they do not.
+  bool beside(const Arg& o, int64_t offset) const {
+    if (dim() < 2 || o.dim() < 2) return false;
+    const int64_t pitch = t->stride(0) * static_cast<int64_t>(t->element_size()), mine = row_bytes(), other = o.row_bytes();
+    if (pitch <= 0 || pitch != o.t->stride(0) * static_cast<int64_t>(o.t->element_size()) || mine == 0 || other == 0) return false;
+    const int64_t at = (offset % pitch + pitch) % pitch;  // of the other's row behind the start of mine
+    return at >= mine && at + other <= pitch;
+  }
   void apart(const Arg& o) const {
     if (!o) return;
     const auto a = span(), b = o.span();
-    if (a.first < b.second && b.first < a.second) refuse(std::string(name) + " overlaps " + o.name);
+    if (a.first < b.second && b.first < a.second && !beside(o, b.first - a.first))
+      refuse(std::string(name) + " overlaps " + o.name);
   }
 };
 

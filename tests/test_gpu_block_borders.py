@@ -359,3 +359,29 @@ def test_forward_mode_tangents_are_refused(cuda):
                 api.causal_conv(fw.make_dual(x, torch.ones_like(x)), w)
             assert e.value.code == _lib.E_INVALID and "gradient" in str(e.value)
         api.causal_conv(x, w)
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+def test_an_output_in_the_other_half_of_the_rows(cuda, kind):
+    """Halves of one buffer's rows do not overlap, although their spans do."""
+    p = ssm_inputs(20, 32, 16, 1, kind, 5, 1)
+    d = {k: v.to(cuda) for k, v in p.items()}
+    w = torch.randn(32, 4, device=cuda)
+    wide = torch.cat((d["x"], torch.zeros_like(d["x"])), 1)
+    left, right = wide[:, :32], wide[:, 32:]
+    assert torch.equal(api.causal_conv(left, w, out=right), api.causal_conv(d["x"], w))
+    scan = (d["dt"], d["A"], d["B"], d["C"])
+    want = api.selective_scan(d["x"], *scan, state=d["state"].clone())
+    assert torch.equal(api.selective_scan(left, *scan, state=d["state"], out=right), want) and torch.equal(left, d["x"])
+    q, s = api.add_rmsnorm_quant(d["x"], torch.ones(32, device=cuda), right.clone())
+    gq, gs = api.add_rmsnorm_quant(left, torch.ones(32, device=cuda), right)
+    assert torch.equal(gq, q) and torch.equal(gs, s)
+    for out in (wide[:, 31:63], wide[:, 1:33], wide[:, :32]):  # one column in common, or all but one, or all
+        with pytest.raises(api.MmfreeError) as e:
+            api.causal_conv(left, w, out=out)
+        assert "overlaps" in str(e.value)
+    rows = torch.zeros(24, 64, dtype=d["x"].dtype, device=cuda)
+    with pytest.raises(api.MmfreeError):  # the same columns a row further
+        api.causal_conv(rows[:20, :32], w, out=rows[1:21, :32])
+    with pytest.raises(api.MmfreeError):  # other pitches
+        api.causal_conv(rows[:20, :32], w, out=rows.view(-1)[:20 * 48].view(20, 48)[:, 16:])
