@@ -125,8 +125,10 @@ def bind():
         import torch  # noqa: F401  (its shared libraries must be loaded first)
         from importlib.machinery import ExtensionFileLoader
         from importlib.util import module_from_spec, spec_from_file_location
-        if not os.path.exists(_build.BIND):
-            raise ImportError(f"{_build.BIND} is missing: run `python -m matmulfreellmcpu_b200.build`")
+        built, here = _build.bind_built_for(), _build.bind_target()
+        if built != here:
+            what = f"was built for {built}, not for {here}" if built else "is missing"
+            raise ImportError(f"{_build.BIND} {what}: run `python -m matmulfreellmcpu_b200.build`")
         loader = ExtensionFileLoader("mmfree_tensor_ops", _build.BIND)
         m = module_from_spec(spec_from_file_location("mmfree_tensor_ops", _build.BIND, loader=loader))
         loader.exec_module(m)

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import concurrent.futures as cf
 import glob
+import json
 import os
 import shutil
 import subprocess
@@ -101,22 +102,49 @@ def build_cli(force: bool = False) -> str:
 
 
 BIND = os.path.join(LIBDIR, "mmfree_tensor_ops.so")
+BIND_FOR = BIND + ".json"  # the interpreter and torch that it was built for
 BIND_SRC = os.path.join(PKG, "bind", "tensor_ops.cpp")
 
 
-def build_bind(force: bool = False) -> str:
-    """The CPython extension that calls the library on torch tensors (host C++ over the C ABI and
-    the installed torch's headers, rpath to the library)."""
+def bind_target() -> dict:
+    """What the tensor binding is tied to: Python's and torch's binary interfaces."""
     import sysconfig
 
     import torch
+    return {"python": sysconfig.get_config_var("SOABI"), "torch": torch.__version__,
+            "cxx11_abi": int(torch._C._GLIBCXX_USE_CXX11_ABI)}
+
+
+def bind_built_for() -> dict | None:
+    """The target of the binding that is there; None without one."""
+    try:
+        with open(BIND_FOR) as f:
+            return json.load(f) if os.path.exists(BIND) else None
+    except (OSError, ValueError):
+        return None
+
+
+def build_bind(force: bool = False) -> str | None:
+    """The CPython extension that calls the library on torch tensors (host C++ over the C ABI and
+    the installed torch's headers, rpath to the library). Without torch it is left out: the C
+    library and the CLI do not need it."""
+    import sysconfig
+    try:
+        import torch
+    except ImportError as e:
+        sys.stderr.write(f"tensor binding not built: torch cannot be imported ({e})\n")
+        return None
+    root = os.path.dirname(torch.__file__)
+    if not os.path.isdir(os.path.join(root, "include", "ATen")):
+        sys.stderr.write(f"tensor binding not built: no torch headers under {root}\n")
+        return None
     deps = [BIND_SRC, LIB, os.path.join(INCLUDE, "mmfree_cuda.h")]
-    if force or not os.path.exists(BIND) or os.path.getmtime(BIND) < max(map(os.path.getmtime, deps)):
-        root = os.path.dirname(torch.__file__)
+    target = bind_target()
+    if force or bind_built_for() != target or os.path.getmtime(BIND) < max(map(os.path.getmtime, deps)):
         cuda = os.path.dirname(os.path.dirname(nvcc()))
         cxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else "g++"
         cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + INCLUDE,
+               f"-D_GLIBCXX_USE_CXX11_ABI={target['cxx11_abi']}", "-I" + INCLUDE,
                "-isystem", os.path.join(root, "include"),
                "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
                "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda, "include"),
@@ -125,6 +153,8 @@ def build_bind(force: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"tensor binding build failed:\n{r.stdout}\n{r.stderr}")
+        with open(BIND_FOR, "w") as f:
+            json.dump(target, f)
     return BIND
 
 
