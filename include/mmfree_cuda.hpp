@@ -152,6 +152,21 @@ inline void rmsnorm_swishgate(float* out, const float* g, const float* o, const 
 }
 
 // The operators of a block with a selective scan (mmfree_cuda.h describes the arguments).
+inline void add_rmsnorm_quant(void* codes, float* scales, const void* x, std::size_t ldx,
+                              void* residual, std::size_t ld_res, const float* weight,
+                              std::size_t rows, std::size_t cols, float eps, int type,
+                              int code_type, std::size_t group = 0, void* stream = nullptr) {
+  check(mmfree_cuda_add_rmsnorm_quant(codes, scales, x, ldx, residual, ld_res, weight, rows, cols,
+                                      eps, type, code_type, group, stream));
+}
+inline void int4_matvec(void* out, const void* x, std::size_t ldx, const float* x_scales,
+                        const std::uint8_t* codes, std::size_t ld_codes, const void* scales,
+                        const std::uint8_t* zeros, std::size_t rows, std::size_t in_dim,
+                        std::size_t out_dim, std::size_t group, std::size_t x_group, int x_type,
+                        int scale_type, int out_type, void* stream = nullptr) {
+  check(mmfree_cuda_int4_matvec(out, x, ldx, x_scales, codes, ld_codes, scales, zeros, rows, in_dim,
+                                out_dim, group, x_group, x_type, scale_type, out_type, stream));
+}
 inline void causal_conv(const mmfree_cuda_conv_args& a, void* stream = nullptr) {
   check(mmfree_cuda_causal_conv(&a, stream));
 }
