@@ -201,7 +201,7 @@ __device__ __forceinline__ float get_out(const void* p, int type, int64_t i) {
 // Outputs of fp32 rows that came out as NaN, once more from the definition in 64 bits, each by the thread that stored it. An
 // infinity's first part is the infinity and its second infinity minus infinity, so its row's outputs are all NaN at first;
 // telling it apart where rows are cut cost every call 8 to 19%.
-__device__ __noinline__ void nan_outputs(const Int4Args& a, int splits, int m0, int live) {
+__device__ __forceinline__ void nan_outputs(const Int4Args& a, int splits, int m0, int live) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.x % splits;
   for (int64_t n = static_cast<int64_t>(blockIdx.x / splits) * 32 + lane; n < a.N; n += static_cast<int64_t>(gridDim.x / splits) * 32)
     for (int m = rank * kWarps + warp; m < live; m += splits * kWarps) {
@@ -227,7 +227,7 @@ __device__ __noinline__ void nan_outputs(const Int4Args& a, int splits, int m0, 
 // touches are copied (a chunk with a byte of the row in it can be read as a whole) and its words put together from
 // two, shifted by the row's own offset.
 template <int kType, int kTiles, bool kAligned>
-__global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCtas) int4_kernel(const __grid_constant__ Int4Args a, int splits, int m0, bool xvec, uint32_t group_inverse) {
+__global__ void __launch_bounds__(32 * kWarps, Int4Shape<kTiles, kAligned>::kCtas) int4_kernel(Int4Args a, int splits, int m0, bool xvec, uint32_t group_inverse) {
   using X = RowType<kType>;
   using S = Int4Shape<kTiles, kAligned>;
   constexpr int kBlocks = S::kBlocks, kRows = S::kRows, kCols = S::kCols, kChunks = S::kChunks, kStages = S::kStages;
