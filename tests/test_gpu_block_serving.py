@@ -138,3 +138,90 @@ def test_convolutions_of_many_tiles(cuda, kind):
         close(out.cpu()[inside], want[inside], bound[inside], f"{len(lens)} sequences")
         assert (out.cpu()[~inside] == SENTINEL).all() and torch.equal(st.cpu(), new)
     api.kernel_status()
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+def test_rows_farther_apart_than_32_bits(cuda, kind):
+    """Row pitches with which the last rows lie behind 2^32 elements."""
+    dtype = R.TYPES[kind]
+    rows, pitch, channels = 37, 1 << 27, 40
+    wide = torch.empty(rows * pitch, dtype=dtype, device=cuda).view(rows, pitch)
+    p = ssm_inputs(rows, channels, 16, 1, kind, 5, 1)
+    p["B"], p["C"] = p["B"][:, 0], p["C"][:, 0]
+    far = {}
+    for i, k in enumerate(("x", "dt", "z", "B", "C")):
+        far[k] = wide[:, 64 * i:64 * i + p[k].shape[1]]
+        far[k].copy_(p[k])
+    out = wide[:, 512:512 + channels]
+    d = {k: v.to(cuda) for k, v in p.items()}
+    scan = lambda q, st, o: api.selective_scan(q["x"], q["dt"], d["A"], q["B"], q["C"], d["D"], q["z"], d["dt_bias"], state=st, out=o)  # noqa: E731
+    s1, s2 = d["state"].clone(), d["state"].clone()
+    assert torch.equal(scan(far, s1, out), scan(d, s2, None)) and torch.equal(s1, s2)
+    pool = torch.randn(rows, channels, 16, device=cuda)
+    step = lambda q, st, o: api.selective_step(q["x"], q["dt"], d["A"], q["B"], q["C"], st, d["D"], q["z"], d["dt_bias"], out=o)  # noqa: E731
+    s1, s2 = pool.clone(), pool.clone()
+    assert torch.equal(step(far, s1, out), step(d, s2, None)) and torch.equal(s1, s2)
+    w = torch.randn(channels, 4, device=cuda)
+    assert torch.equal(api.causal_conv(far["x"], w, out=out), api.causal_conv(d["x"], w))
+    s1 = torch.randn(rows, 3, channels, device=cuda).to(dtype)
+    s2 = s1.clone()
+    assert torch.equal(api.causal_conv_step(far["x"], w, s1, out=out), api.causal_conv_step(d["x"], w, s2)) and torch.equal(s1, s2)
+    ones = torch.ones(channels, device=cuda)
+    r = d["dt"].clone()
+    for a, b in zip(api.add_rmsnorm_quant(far["x"], ones, far["dt"]), api.add_rmsnorm_quant(d["x"], ones, r)):
+        assert torch.equal(a.float(), b.float())
+    assert torch.equal(far["dt"], r)
+    _, codes, scales, _, _ = int4_inputs(1, channels, 60, 32, False, "fp32", 3)
+    cd, sd = dev(cuda, codes, scales)
+    want = api.int4_matvec(d["x"], cd, sd, 32)
+    assert torch.equal(api.int4_matvec(far["x"], cd, sd, 32), want)
+    bytes_ = wide.view(-1).view(torch.uint8)
+    for start in (0, 5):  # rows of codes at aligned and at odd addresses
+        rows_of = bytes_[:60 * (1 << 27)].view(60, 1 << 27)[:, 4096 + start:4096 + start + codes.shape[1]]
+        rows_of.copy_(codes)
+        assert torch.equal(api.int4_matvec(d["x"], rows_of, sd, 32), want)
+    api.kernel_status()
+
+
+def test_every_operator_on_two_other_streams_at_once_and_captured(cuda):
+    """Calls with ``stream``, on two streams that overlap and in graphs of two streams, give what the current stream gives: a
+    split scan, products over a cluster, rows whose scales and outputs are taken again, and the steps."""
+    p = {k: v.to(cuda) for k, v in ssm_inputs(2000, 48, 16, 1, "fp32", 5, 1).items()}
+    w, x = torch.randn(48, 4, device=cuda), torch.randn(9, 5632, device=cuda)
+    x[3] *= 1e25
+    x[5, 7] = torch.inf
+    _, codes, scales, _, _ = int4_inputs(1, 5632, 160, 64, False, "fp32", 3)
+    cd, sd = dev(cuda, codes, scales)
+    rows = slice(0, 40)
+
+    def run(stream=None):
+        st, conv, pool = p["state"].clone(), torch.zeros(40, 3, 48, device=cuda), torch.ones(40, 48, 16, device=cuda)
+        y = api.selective_scan(p["x"], p["dt"], p["A"], p["B"], p["C"], p["D"], p["z"], p["dt_bias"], state=st, stream=stream)
+        c = api.causal_conv(p["x"], w, stream=stream)
+        cs = api.causal_conv_step(p["x"][rows], w, conv, stream=stream)
+        s = api.selective_step(p["x"][rows], p["dt"][rows], p["A"], p["B"][rows], p["C"][rows], pool, stream=stream)
+        q, qs = api.add_rmsnorm_quant(x, torch.ones(5632, device=cuda), eps=0.0, stream=stream)
+        m = api.int4_matvec(x, cd, sd, 64, stream=stream)
+        return y, st, c, cs, conv, s, pool, q, qs.nan_to_num(7.0), m.nan_to_num(7.0)
+
+    want = run()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(3):
+        for side in streams:
+            with torch.cuda.stream(side):
+                got.append(run(side))
+    graphs = []
+    for side in streams:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs = run()
+        graphs.append((side, graph, outs))
+    for side, graph, _ in graphs:
+        with torch.cuda.stream(side):
+            graph.replay()
+    torch.cuda.synchronize()
+    for outs in got + [g[2] for g in graphs]:
+        for i, (a, b) in enumerate(zip(outs, want)):
+            assert torch.equal(a, b), i
