@@ -391,7 +391,8 @@ def causal_conv(x, weight, bias=None, state=None, seq_starts=None, slots=None, s
     ``x`` [tokens, channels] float32, bfloat16 or float16; ``weight`` float32 [channels, width],
     width 2 to 8, the newest input's tap last; ``bias`` float32 [channels]. ``seq_starts`` int32
     [sequences + 1] on the device: the first row of each sequence and the row behind the last
-    (without: one sequence); rows outside the sequences are left as they were in ``out``.
+    (without: one sequence); rows outside the sequences are left as they were in ``out`` (and are
+    undefined in an output that the call makes).
     ``state`` [states, width - 1, channels] of ``x``'s type: the inputs before each sequence,
     oldest first, updated in place (without: zeros). ``slots`` int32 [sequences]: the state of
     each sequence (they must differ; a negative one marks a sequence that is left out).

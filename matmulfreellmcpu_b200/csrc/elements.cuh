@@ -94,7 +94,7 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 constexpr float kLog2E = 1.44269504088896341f;
 
-// 2^v and 1 / v by the special-function unit (relative errors of at most 2^-22 and 2^-23).
+// 2^v and 1 / v by the special-function unit (relative errors of at most 2^-22 and 2^-23; below 2^-126 both are 0).
 __device__ __forceinline__ float ex2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));

@@ -200,7 +200,7 @@ __device__ __forceinline__ float get_out(const void* p, int type, int64_t i) {
 
 // Outputs of fp32 rows that came out as NaN, once more from the definition in 64 bits, each by the thread that stored it. An
 // infinity's first part is the infinity and its second infinity minus infinity, so its row's outputs are all NaN at first;
-// telling it apart where rows are cut cost every call 8 to 19%.
+// telling it apart where rows are cut made calls 8 to 19% slower.
 __device__ __forceinline__ void nan_outputs(const Int4Args& a, int splits, int m0, int live) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.x % splits;
   for (int64_t n = static_cast<int64_t>(blockIdx.x / splits) * 32 + lane; n < a.N; n += static_cast<int64_t>(gridDim.x / splits) * 32)

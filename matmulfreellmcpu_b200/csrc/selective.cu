@@ -269,8 +269,9 @@ cudaError_t conv_any(const mmfree_cuda_conv_args& a, bool step, cudaStream_t s) 
 // ---- selective scan --------------------------------------------------------------------------
 
 // softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) <= 1, with log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1/3,
-// by its series 2 (s + s^3/3 + s^5/5 + ...): the first term left out is below 2^-25 of the sum. Exact to a few
-// steps for all v, where log(1 + e) rounded first would lose small e. Two special-function operations.
+// by its series 2 (s + s^3/3 + s^5/5 + ...): the first term left out is below 2^-25 of the sum. For v >= 0 off by a few
+// steps; for v < 0 by (6 + |v|) 2^-24 of the value at most, since exp's argument |v| log2(e) is rounded once, and 0 below
+// -87.3. (log(1 + e) rounded first would lose small e altogether.) Two special-function operations.
 __device__ __forceinline__ float softplus_f32(float v) {
   const float e = ex2(-fabsf(v) * kLog2E);
   const float s = e * rcp(2.0f + e), q = s * s;
@@ -290,9 +291,9 @@ __device__ __forceinline__ float softplus_f32(float v) {
 __device__ __forceinline__ float finite_rate(float v) { return isinf(v) ? copysignf(3.402823466e38f, v) : v; }
 
 // One token of each of kStreams streams: `lanes` lanes (a power of two) a channel, kStates neighbouring states a lane,
-// kVec: read and written by 16 bytes. Bound by its issue slots (67% busy at 256 streams, 3.2 TB/s) and by how many of
-// the state's bytes are in flight together: four streams a thread where there are enough. Every lane repeats its channel's softplus and gate, which costs less than passing
-// them on.
+// kVec: read and written by 16 bytes. Bound by its issue slots (78% busy at 256 streams of 4096 x 16: 39 us, 3.6 TB/s) and by
+// how many of the state's bytes are in flight together: four streams a thread where there are enough. Every lane repeats its
+// channel's softplus and gate.
 template <typename T, int kStates, int kStreams, bool kVec>
 __global__ void __launch_bounds__(256) step_kernel(mmfree_cuda_ssm_args a, int lanes) {
   const int64_t channels = static_cast<int64_t>(a.channels), seqs = static_cast<int64_t>(a.seqs);
@@ -471,7 +472,7 @@ struct ScanShape {
 // run without outputs first, then every piece but the first starts from the states and sums of those before it, read
 // from their shared memory. Two passes for a sequence, each over 1 / splits of it.
 // Bound by the exponentials, one for each token, channel and state: 16 a clock and SM, 385 us with the helpers' for
-// 16384 tokens x 5120 channels x 16 states, where the kernel takes 646 us; the special-function unit is busy 60% of the
+// 16384 tokens x 5120 channels x 16 states, where the kernel takes 647 us; the special-function unit is busy 60% of the
 // time, the rest goes to the two halves' waits for each other and for its latency. An eighth or a quarter of the
 // exponentials as polynomials on the multiply-add pipe changed nothing (663 and 693 against 657 us), nor did more CTAs an SM.
 // What a turn of the recurrence reads from shared memory bounds it next to the special-function unit (128 bytes of
@@ -829,8 +830,9 @@ cudaError_t scan_launch(const mmfree_cuda_ssm_args& a, int sms, cudaStream_t s) 
   constexpr size_t kSmem = sizeof(typename S::Shared);
   const int blocks = static_cast<int>(ceil_div(static_cast<int64_t>(a.channels / a.groups), S::kChannels));
   // Few CTAs and long sequences: clusters of 8 or 4 split each sequence, as many as two CTAs an SM hold. One sequence of
-  // 8192 tokens x 1024 channels (bf16, 32 CTAs): 334 us in one piece, 145 us in 8; 2048 x 2048 (64 CTAs): 86.5 us in one
-  // piece, 74.8 us in 4.
+  // 8192 tokens x 1024 channels (bf16, 32 CTAs): 334 us in one piece, 144 us in 8; 2048 x 2048 (64 CTAs): 86.5 us in one
+  // piece, 74.7 us in 4. The host knows the sequences' mean length alone, and goes by it here and in scan_states: a long
+  // prompt among many short sequences is not split.
   const int64_t ctas = static_cast<int64_t>(blocks) * static_cast<int64_t>(a.groups * a.seqs);
   const bool long_ones = a.tokens / a.seqs >= 512;
   const int splits = !S::kMaySplit || !long_ones ? 1 : ctas * 4 <= sms ? 8 : ctas * 2 <= sms ? 4 : 1;
@@ -860,8 +862,9 @@ cudaError_t scan_states(const mmfree_cuda_ssm_args& a, int sms, cudaStream_t s) 
   if (a.states <= 16) {
     // Short sequences on many CTAs: two channels a lane (half the reads of B and C) and tiles of 16 tokens, which leave
     // less behind a sequence's end: 300 tokens in 16 sequences x 2048 channels (fp32) take 14.3 against 16.7 us. Long
-    // ones the other way: 16384 tokens in 8 sequences x 5120 channels (bf16) 646 against 657 us, one sequence of
-    // 4099 x 4096 160 against 203 us.
+    // ones the other way: 16384 tokens in 8 sequences x 5120 channels (bf16) 647 against 657 us, one sequence of
+    // 4099 x 4096 160 against 203 us. By the mean length: 63 single tokens and a prompt of 4033 x 4096 (bf16) come here and
+    // take 417 us, the prompt alone 164 us.
     if (static_cast<int64_t>(a.channels * a.seqs) >= 32 * 3 * static_cast<int64_t>(sms) && a.tokens / a.seqs < 512)
       return scan_launch<ScanShape<T, 4, 4, 2, 16, 64, 64, 4, kBytes>>(a, sms, s);
     return scan_launch<ScanShape<T, 4, 4, 1, 32, 128, 128, 2, kBytes>>(a, sms, s);
@@ -889,7 +892,7 @@ template <typename T, int kStates, bool kVec>
 cudaError_t step_launch(const mmfree_cuda_ssm_args& a, int lanes, cudaStream_t s) {
   const unsigned blocks = static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.channels) * lanes, 256));
   // four streams a thread where one stream a thread would be more threads than the 148 SMs hold at once (4096 x 16
-  // states: 64 streams 13.4 against 15.9 us, 256 streams 45.3 against 57.5 us)
+  // states, with slots, captured: 64 streams 11.2 against 14.8 us, 256 streams 39.2 against 53.5 us)
   if (static_cast<int64_t>(blocks) * static_cast<int64_t>(a.seqs) > 148 * 8)
     return launch_k(step_kernel<T, kStates, 4, kVec>, dim3(blocks, static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.seqs), 4))), dim3(256), 0, s, false, a, lanes);
   return launch_k(step_kernel<T, kStates, 1, kVec>, dim3(blocks, static_cast<unsigned>(a.seqs)), dim3(256), 0, s, false, a, lanes);
