@@ -76,12 +76,12 @@ int mmfree_cuda_bitlinear(float* out, const float* x, const float* norm_weight,
  * mmfree_cuda_bitlinear_cluster, mmfree_cuda_bitlinear_noalloc, mmfree_cuda_int4_matvec,
  * mmfree_cuda_causal_conv, mmfree_cuda_selective_scan and their steps). They return once their
  * kernels are queued; a failure inside a kernel (a bounded wait that gave up, a sequence start,
- * slot or zero point out of range) is recorded in a device error word instead. This call synchronizes `stream` (the stream those calls used),
- * reads and clears the calling device's words and returns MMFREE_OK, or MMFREE_E_TIMEOUT when
- * a call since the last check failed -- the outputs of those calls are then undefined -- or
- * MMFREE_E_RANGE when one met a bad sequence start, slot or zero point. It
- * allocates nothing. No reference counterpart: the reference kernels are synchronous host
- * code that cannot time out. */
+ * slot or zero point out of range) is recorded in a device error word instead. This call
+ * synchronizes `stream` (the stream those calls used), reads and clears the calling device's
+ * words and returns MMFREE_OK, or MMFREE_E_TIMEOUT when a call since the last check failed --
+ * the outputs of those calls are then undefined -- or MMFREE_E_RANGE when one met a bad
+ * sequence start, slot or zero point. It allocates nothing. No reference counterpart: the
+ * reference kernels are synchronous host code that cannot time out. */
 int mmfree_cuda_kernel_status(void* stream);
 
 /* Diagnostic switch: the number of polls after which the BitLinear prologue's wait for its
@@ -221,7 +221,8 @@ int mmfree_cuda_add_rmsnorm_quant(void* codes, float* scales, const void* x, siz
  * or F16 with x_scales NULL, or S8 / E4M3 codes with the scales of
  * mmfree_cuda_add_rmsnorm_quant: x_scales [rows] with x_group 0, or [rows, ceil(in_dim /
  * group)] with x_group == group. out [rows, out_dim] contiguous of out_type (F32, BF16 or
- * F16). Sums are in fp32 (whole numbers within a group for S8 rows). Meant for a few rows (1 to 32), right for any number. */
+ * F16). Sums are in fp32 (whole numbers within a group for S8 rows). Meant for a few rows (1 to
+ * 32), right for any number. */
 int mmfree_cuda_int4_matvec(void* out, const void* x, size_t ldx, const float* x_scales,
                             const uint8_t* codes, size_t ld_codes, const void* scales,
                             const uint8_t* zeros, size_t rows, size_t in_dim, size_t out_dim,

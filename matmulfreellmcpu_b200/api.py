@@ -418,8 +418,8 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus: bo
     ``x``, ``dt`` and ``z`` [tokens, channels], ``B`` and ``C`` [tokens, states] or [tokens,
     groups, states], all of one type (float32, bfloat16 or float16); ``A`` [channels, states],
     ``D`` and ``dt_bias`` [channels] and ``state`` [states, channels, A's columns] float32, the
-    state updated in place (without: zeros). An infinity in ``A`` counts as the largest finite number. ``seq_starts``, ``slots`` and ``out`` as in
-    :func:`causal_conv`. Returns y of ``x``'s type."""
+    state updated in place (without: zeros). An infinity in ``A`` counts as the largest finite
+    number. ``seq_starts``, ``slots`` and ``out`` as in :func:`causal_conv`. Returns y of ``x``'s type."""
     return bind().selective(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state, seq_starts, slots, out,
                             stream, False)
 

@@ -424,12 +424,12 @@ int mmfree_cuda_kernel_status(void* stream) {
     if (f & kErrTimeout)
       throw TimeoutError("a bounded wait inside a BitLinear kernel gave up: the outputs of the "
                          "kernel calls since the last status check are undefined");
+    std::string range;
+    if (sequence & kErrRange)
+      range = "a sequence start or slot given to causal_conv or selective_scan is out of range or out of order";
     if (zero_point & kErrRange)
-      throw std::out_of_range("a zero point given to int4_matvec with F32 or BF16 rows since the "
-                              "last status check is above 127");
-    if (f & kErrRange)
-      throw std::out_of_range("a sequence start or slot given to causal_conv or selective_scan "
-                              "since the last status check is out of range or out of order");
+      range += std::string(range.empty() ? "" : "; ") + "a zero point given to int4_matvec with F32 or BF16 rows is above 127";
+    if (!range.empty()) throw std::out_of_range("since the last status check: " + range);
     if (f) throw std::runtime_error("device error flag set");
   });
 }

@@ -216,6 +216,7 @@ __device__ __forceinline__ void nan_outputs(const Int4Args& a, int splits, int m
         double part = 0.0;
         for (int k = g * a.group; k < stop; ++k) part += static_cast<double>((codes[k >> 1] >> (4 * (k & 1)) & 15) - zero) * x[k];
         total += part * get_out(a.scales, a.scale_type, of);
+        if (isnan(total)) break;  // whatever follows
       }
       put_out(a.out, a.out_type, at, static_cast<float>(total));
     }

@@ -385,3 +385,15 @@ def test_an_output_in_the_other_half_of_the_rows(cuda, kind):
         api.causal_conv(rows[:20, :32], w, out=rows[1:21, :32])
     with pytest.raises(api.MmfreeError):  # other pitches
         api.causal_conv(rows[:20, :32], w, out=rows.view(-1)[:20 * 48].view(20, 48)[:, 16:])
+
+
+def test_one_status_names_both_kinds_of_error(cuda):
+    x, w, st = torch.randn(2, 64, device=cuda), torch.randn(64, 4, device=cuda), torch.zeros(2, 3, 64, device=cuda)
+    codes, scales = torch.zeros(8, 32, dtype=torch.uint8, device=cuda), torch.ones(8, 2, device=cuda)
+    api.kernel_status()
+    api.int4_matvec(x, codes, scales, 32, zeros=torch.full((8, 2), 200, dtype=torch.uint8, device=cuda))
+    api.causal_conv_step(x, w, st, slots=torch.tensor([0, 5], dtype=torch.int32, device=cuda))
+    with pytest.raises(api.MmfreeError) as e:
+        api.kernel_status()
+    assert e.value.code == _lib.E_RANGE and "zero point" in str(e.value) and "slot" in str(e.value)
+    api.kernel_status()
