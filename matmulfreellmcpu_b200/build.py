@@ -131,7 +131,7 @@ def build_bind(force: bool = False) -> str | None:
     import sysconfig
     try:
         import torch
-    except ImportError as e:
+    except (ImportError, OSError) as e:  # not there, or a library of its own is not
         sys.stderr.write(f"tensor binding not built: torch cannot be imported ({e})\n")
         return None
     root = os.path.dirname(torch.__file__)
